@@ -351,6 +351,70 @@ int slg_thermo_soft_fwd(const float* x, const float* thr, int64_t B, int64_t F, 
 int slg_thermo_soft_bwd(const float* x, const float* thr, const float* g, int64_t B, int64_t F,
                         int32_t T, float scale, float* gx, float* gthr, void* stream);
 
+/* ------------------------------------------- token input and output, training memory
+ *
+ * Element types of the entry points below (32-bit arithmetic on all of them). */
+#define SLG_DT_F32 0
+#define SLG_DT_BF16 1
+#define SLG_DT_F16 2
+
+/* Token embedding: out[i, :] = scale * weight[ids[i], :], weight [V, D] row-major, out
+ * [N, D] (16-byte aligned) of the same type.  ids are int32 (ids64 = 0) or int64 (1); an
+ * id outside [0, V) gives a row of NaN and reads nothing.  N, V < 2^31. */
+int slg_embed_fwd(const void* ids, int32_t ids64, int64_t N, const void* weight, int32_t dtype,
+                  int64_t V, int64_t D, float scale, void* out, void* stream);
+
+/* Its gradient: gw[v, :] = scale * sum of g[i, :] over ids[i] == v, every row written
+ * (zero where no id names it), 32-bit sums in a fixed order (tokens sorted by a stable
+ * sort, so the result is the same from run to run), rounded once.  Ids equal to
+ * padding_idx (pass -1 for none) or outside [0, V) add nothing. */
+int64_t slg_embed_bwd_workspace_bytes(int64_t N, int64_t V, int64_t D, int32_t dtype);
+int slg_embed_bwd(const void* ids, int32_t ids64, int64_t N, const void* g, int32_t dtype,
+                  int64_t V, int64_t D, float scale, int64_t padding_idx, void* gw,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+
+/* 8-bit activation checkpoints.  A row is cut into blocks of SLG_CKPT_BLOCK columns; a
+ * block keeps (lo, step) = (min, (max - lo) * fl(1/255)) in fp32 and one byte per value,
+ *   code = rint((x - lo) * (255 / (max - lo))),  value read back = code * step + lo,
+ * each operation rounded by itself.  step < 2^-100 is kept as 0 (code 0); a block with a
+ * value that is not finite, or whose max - lo overflows, reads back as NaN.
+ * x [rows, cols] with row stride ldx; codes [rows, ldc] (ldc a multiple of 4, >= cols);
+ * bounds [rows, ceil(cols / SLG_CKPT_BLOCK), 2] fp32. */
+#define SLG_CKPT_BLOCK 128
+int slg_ckpt_store(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ldx,
+                   uint8_t* codes, int64_t ldc, float* bounds, void* stream);
+int slg_ckpt_load(const uint8_t* codes, int64_t ldc, const float* bounds, int64_t rows,
+                  int64_t cols, void* x, int32_t dtype, int64_t ldx, void* stream);
+
+/* One step of beam search.  logits [B * beams, V] with row stride ldx, scores [B, beams]
+ * (sums of log probabilities so far; -inf for a beam that is not in use).  Candidate
+ * (b, v) has (x - max_b) - log(sum exp(x - max_b)) + scores[b]; a beam with finished[b]
+ * != 0 has the one candidate (b, eos) at scores[b].  The `width` best of each entry come
+ * out in order, equal values by the lowest b * V + v: their values, beams (parents), tokens and,
+ * when out_finished is given, finished[parent] || token == eos.  NaN logits count as
+ * masked (-inf), +inf as the largest finite value; masked candidates (value -inf) come
+ * last.  beams, width <= SLG_BEAM_MAX; finished and out_finished may be NULL. */
+#define SLG_BEAM_MAX 32
+int64_t slg_beam_step_workspace_bytes(int64_t B, int32_t beams, int64_t V, int32_t width);
+int slg_beam_step(const void* logits, int32_t dtype, int64_t B, int32_t beams, int64_t V,
+                  int64_t ldx, const float* scores, const uint8_t* finished, int32_t eos,
+                  int32_t width, float* out_scores, int64_t* parents, int64_t* tokens,
+                  uint8_t* out_finished, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Decoder state after a step: sample r = e * width + n of `out` is sample
+ * e * beams + parents[e, n] of `in` (a parent outside [0, beams) reads beam 0).
+ * rows: [samples, row_bytes] of any type; features: feature-major fp32 [F, ld]; packed:
+ * bit-packed [F, ld] uint64.  Padding columns and bits are written 0.  `out` must not
+ * overlap `in`. */
+int slg_beam_reorder_rows(const void* in, int64_t row_bytes, const int64_t* parents, int64_t B,
+                          int32_t beams, int32_t width, void* out, void* stream);
+int slg_beam_reorder_features(const float* in, int64_t F, int64_t ldi, const int64_t* parents,
+                              int64_t B, int32_t beams, int32_t width, float* out, int64_t ldo,
+                              void* stream);
+int slg_beam_reorder_packed(const uint64_t* in, int64_t F, int64_t ldi, const int64_t* parents,
+                            int64_t B, int32_t beams, int32_t width, uint64_t* out, int64_t ldo,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -19,6 +19,9 @@ from .layers import (LogicLayer, WARPLayer, WARPLayerN, LUTkLayer, LUTNodeLayer,
 from .models import (LogicNet, WARPNet, WARPNetN, LUTkNet, LUTNodeNet, LogicConvNet,
                      LogicTreeNet)
 from .encoders import LearnedThermometerEncoder
+from .checkpoints import checkpoint8, checkpoint8_store, Checkpoint8
+from .tokens import token_embedding, TokenEmbedding
+from .beam import beam_step, beam_reorder, BeamStep
 from .data import (binarize_spatial, MNIST_THRESH, SEVEN_THRESH, FOUR_THRESH, FIVE_THRESH,
                    CIFAR3_THRESH, EDGE_THRESH)
 
@@ -31,6 +34,9 @@ __all__ = [
     "ConvLogicTree", "ConvLogicLayer", "OrPool",
     "LogicNet", "WARPNet", "WARPNetN", "LUTkNet", "LUTNodeNet", "LogicConvNet", "LogicTreeNet",
     "LearnedThermometerEncoder",
+    "checkpoint8", "checkpoint8_store", "Checkpoint8",
+    "token_embedding", "TokenEmbedding",
+    "beam_step", "beam_reorder", "BeamStep",
     "binarize_spatial", "MNIST_THRESH", "SEVEN_THRESH", "FOUR_THRESH", "FIVE_THRESH",
     "CIFAR3_THRESH", "EDGE_THRESH",
 ]

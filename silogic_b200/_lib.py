@@ -56,6 +56,15 @@ _SIGS = {
     "slg_conv_soft_bwd": [_p, _i64, _i64, _i64, _i64, _p, _p, _i32, _i32, _i32, _i32, _i32, _p,
                           _i32, _f32, _i32, _i32, _i64, _i64, _i32, _p, _p, _p, _p, _p, _p, _i64,
                           _p],
+    "slg_embed_fwd": [_p, _i32, _i64, _p, _i32, _i64, _i64, _f32, _p, _p],
+    "slg_embed_bwd": [_p, _i32, _i64, _p, _i32, _i64, _i64, _f32, _i64, _p, _p, _i64, _p],
+    "slg_ckpt_store": [_p, _i32, _i64, _i64, _i64, _p, _i64, _p, _p],
+    "slg_ckpt_load": [_p, _i64, _p, _i64, _i64, _p, _i32, _i64, _p],
+    "slg_beam_step": [_p, _i32, _i64, _i32, _i64, _i64, _p, _p, _i32, _i32, _p, _p, _p, _p, _p,
+                      _i64, _p],
+    "slg_beam_reorder_rows": [_p, _i64, _p, _i64, _i32, _i32, _p, _p],
+    "slg_beam_reorder_features": [_p, _i64, _i64, _p, _i64, _i32, _i32, _p, _i64, _p],
+    "slg_beam_reorder_packed": [_p, _i64, _i64, _p, _i64, _i32, _i32, _p, _i64, _p],
 }
 # entry points that do not return a status
 _RESTYPES = {
@@ -63,6 +72,8 @@ _RESTYPES = {
     "slg_fc_soft_workspace_bytes": ([_i64, _i32, _i32, _i32, _i64], ctypes.c_int64),
     "slg_conv_soft_workspace_bytes": ([_i64, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
                                        _i64], ctypes.c_int64),
+    "slg_embed_bwd_workspace_bytes": ([_i64, _i64, _i64, _i32], ctypes.c_int64),
+    "slg_beam_step_workspace_bytes": ([_i64, _i32, _i64, _i32], ctypes.c_int64),
 }
 
 _lib = None

@@ -285,3 +285,102 @@ def thermo_soft_bwd(x: Tensor, thr: Tensor, g: Tensor, scale: float,
 @thermo_soft_bwd.register_fake
 def _(x, thr, g, scale, need_gx):
     return (torch.empty_like(x) if need_gx else x.new_empty((0,))), torch.empty_like(thr)
+
+
+# ------------------------------------------------- token embedding (sorted gradient)
+DTYPE_ID = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+@_op("embed_fwd")
+def embed_fwd(ids: Tensor, weight: Tensor, scale: float) -> Tensor:
+    """``scale * weight[ids]``: ids int32 / int64 of any shape, weight ``[V, D]``."""
+    V, D = weight.shape
+    out = torch.empty(ids.shape + (D,), dtype=weight.dtype, device=weight.device)
+    call("slg_embed_fwd", ptr(ids), ids.dtype == torch.int64, ids.numel(), ptr(weight),
+         DTYPE_ID[weight.dtype], V, D, scale, ptr(out), stream_ptr(weight.device))
+    return out
+
+
+@embed_fwd.register_fake
+def _(ids, weight, scale):
+    return weight.new_empty(tuple(ids.shape) + (weight.shape[1],))
+
+
+@_op("embed_bwd")
+def embed_bwd(ids: Tensor, g: Tensor, V: int, scale: float, padding_idx: int) -> Tensor:
+    """``[V, D]``: row v = scale * sum of g's rows whose id is v (padding_idx -1: none)."""
+    g = g.contiguous()
+    D = g.shape[-1]
+    N, dt = ids.numel(), DTYPE_ID[g.dtype]
+    gw = torch.empty((V, D), dtype=g.dtype, device=g.device)
+    nbytes = lib().slg_embed_bwd_workspace_bytes(N, V, D, dt)
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=g.device)
+    call("slg_embed_bwd", ptr(ids), ids.dtype == torch.int64, N, ptr(g), dt, V, D, scale,
+         padding_idx, ptr(gw), ptr(ws), nbytes, stream_ptr(g.device))
+    return gw
+
+
+@embed_bwd.register_fake
+def _(ids, g, V, scale, padding_idx):
+    return g.new_empty((V, g.shape[-1]))
+
+
+# --------------------------------------------------- 8-bit activation checkpoints
+CKPT_BLOCK = 128        # columns per (lo, step) pair (SLG_CKPT_BLOCK)
+
+
+@_op("ckpt_store")
+def ckpt_store(x: Tensor) -> Tuple[Tensor, Tensor]:
+    """``[rows, cols]`` (rows may be strided) -> (codes uint8 ``[rows, ldc]``, bounds fp32
+    ``[rows, blocks, 2]``)."""
+    require_cuda(x)
+    if x.stride(1) != 1 or x.stride(0) < x.shape[1]:
+        x = x.contiguous()
+    rows, cols = x.shape
+    codes = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.uint8, device=x.device)
+    bounds = torch.empty((rows, -(-cols // CKPT_BLOCK), 2), dtype=torch.float32, device=x.device)
+    call("slg_ckpt_store", ptr(x), DTYPE_ID[x.dtype], rows, cols, max(x.stride(0), cols), ptr(codes),
+         codes.shape[1], ptr(bounds), stream_ptr(x.device))
+    return codes, bounds
+
+
+@ckpt_store.register_fake
+def _(x):
+    rows, cols = x.shape
+    return (x.new_empty((rows, (cols + 15) // 16 * 16), dtype=torch.uint8),
+            x.new_empty((rows, (cols + CKPT_BLOCK - 1) // CKPT_BLOCK, 2), dtype=torch.float32))
+
+
+@_op("ckpt_load")
+def ckpt_load(codes: Tensor, bounds: Tensor, cols: int, dtype: torch.dtype) -> Tensor:
+    """The ``[rows, cols]`` values that the codes stand for."""
+    require_cuda(codes, bounds)
+    rows = codes.shape[0]
+    x = torch.empty((rows, cols), dtype=dtype, device=codes.device)
+    call("slg_ckpt_load", ptr(codes), codes.shape[1], ptr(bounds), rows, cols, ptr(x),
+         DTYPE_ID[dtype], cols, stream_ptr(codes.device))
+    return x
+
+
+@ckpt_load.register_fake
+def _(codes, bounds, cols, dtype):
+    return codes.new_empty((codes.shape[0], cols), dtype=dtype)
+
+
+@_op("fc_soft_bwd_ckpt")
+def fc_soft_bwd_ckpt(codes: Tensor, bounds: Tensor, ldb: int, cand: Tensor, conn: Optional[Tensor],
+                     params: Tensor, K: int, ste: int, node: int, arity: int, gate_hard: int,
+                     inv_tau: float, out_dim: int, wire_r: int, gy: Tensor,
+                     need_gx: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    """:func:`fc_soft_bwd` at the activations that an 8-bit checkpoint stands for."""
+    xt = IMPL["ckpt_load"](codes, bounds, ldb, torch.float32)
+    return IMPL["fc_soft_bwd"](xt, cand, conn, params, K, ste, node, arity, gate_hard, inv_tau, out_dim,
+                       wire_r, gy, need_gx)
+
+
+@fc_soft_bwd_ckpt.register_fake
+def _(codes, bounds, ldb, cand, conn, params, K, ste, node, arity, gate_hard, inv_tau, out_dim,
+      wire_r, gy, need_gx):
+    gx = params.new_empty((codes.shape[0], ldb)) if need_gx else params.new_empty((0,))
+    gconn = torch.empty_like(conn) if conn is not None else params.new_empty((0,))
+    return gx, torch.empty_like(params), gconn

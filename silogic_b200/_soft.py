@@ -21,6 +21,15 @@ def ldb_for(B):
     return max(4, (int(B) + 3) // 4 * 4)
 
 
+#: set by :func:`silogic_b200.checkpoint8`: layers keep their input for the backward pass
+#: as 8-bit codes instead of fp32
+CHECKPOINT8 = False
+
+
+def _keep_checkpoint(ctx):
+    return CHECKPOINT8 and any(ctx.needs_input_grad[:3])
+
+
 # ------------------------------------------------------------- transposes
 class ToFeatureMajor(torch.autograd.Function):
     @staticmethod
@@ -106,16 +115,27 @@ class FCSoft(torch.autograd.Function):
         params = params.float().contiguous()
         connc = conn.float().contiguous() if conn is not None else None
         y = op("fc_soft_fwd")(xt, meta["cand"], connc, params, *FCSoft._args(meta))
-        ctx.save_for_backward(xt, params, connc)
+        ctx.ckpt = _keep_checkpoint(ctx)
+        if ctx.ckpt:        # the backward pass works from 8-bit codes; xt itself is let go
+            ctx.save_for_backward(*op("ckpt_store")(xt), params, connc)
+            ctx.ldb = xt.shape[1]
+        else:
+            ctx.save_for_backward(xt, params, connc)
         ctx.meta = meta
         return y
 
     @staticmethod
     def backward(ctx, gy):
-        xt, params, connc = ctx.saved_tensors
         m = ctx.meta
-        gx, gparams, gconn = op("fc_soft_bwd")(xt, m["cand"], connc, params, *FCSoft._args(m), gy,
-                                             bool(ctx.needs_input_grad[0]))
+        need_gx = bool(ctx.needs_input_grad[0])
+        if ctx.ckpt:
+            codes, bounds, params, connc = ctx.saved_tensors
+            gx, gparams, gconn = op("fc_soft_bwd_ckpt")(codes, bounds, ctx.ldb, m["cand"], connc,
+                                                        params, *FCSoft._args(m), gy, need_gx)
+        else:
+            xt, params, connc = ctx.saved_tensors
+            gx, gparams, gconn = op("fc_soft_bwd")(xt, m["cand"], connc, params, *FCSoft._args(m),
+                                                 gy, need_gx)
         return (gx if ctx.needs_input_grad[0] else None, gparams,
                 gconn if connc is not None else None, None)
 
@@ -268,13 +288,22 @@ class ConvSoft(torch.autograd.Function):
         y, arg = op("conv_soft_fwd")(xt, C, H, W, meta["cand"], connc, params,
                                      *ConvSoft._args(meta),
                                    keep)
-        ctx.save_for_backward(xt, params, connc, arg)
+        ctx.ckpt = _keep_checkpoint(ctx)
+        if ctx.ckpt:
+            ctx.save_for_backward(*op("ckpt_store")(xt), params, connc, arg)
+            ctx.ldb = xt.shape[1]
+        else:
+            ctx.save_for_backward(xt, params, connc, arg)
         ctx.meta, ctx.shape = meta, shape
         return y
 
     @staticmethod
     def backward(ctx, gy):
-        xt, params, connc, arg = ctx.saved_tensors
+        if ctx.ckpt:        # the conv kernels read fp32 planes: one block's input at a time
+            codes, bounds, params, connc, arg = ctx.saved_tensors
+            xt = op("ckpt_load")(codes, bounds, ctx.ldb, torch.float32)
+        else:
+            xt, params, connc, arg = ctx.saved_tensors
         m = ctx.meta
         C, H, W = ctx.shape
         if m.get("deterministic") and ctx.needs_input_grad[0]:

@@ -1,0 +1,106 @@
+"""Beam search on token logits: one selection step over beams and vocabulary, and the
+reordering of the decoder's state -- rows, feature-major activations, or the bit-packed
+activations of a hard circuit -- by the chosen beams."""
+from collections import namedtuple
+
+import torch
+
+from . import _hard, _soft
+from ._lib import call, lib, ptr, require_cuda, stream_ptr
+from ._ops import DTYPE_ID
+
+BEAM_MAX = 32           # SLG_BEAM_MAX
+
+#: ``scores`` fp32, ``parents`` and ``tokens`` int64, ``finished`` bool (None without ``eos``),
+#: each ``[B, width]``, best first
+BeamStep = namedtuple("BeamStep", "scores parents tokens finished")
+
+
+@torch.no_grad()
+def beam_step(logits, scores, finished=None, eos=None, width=None):
+    """The ``width`` (default: as many as there are) best continuations of each entry's beams.
+
+    ``logits`` ``[B, beams, V]`` or ``[B * beams, V]`` (float32, bfloat16 or float16; class
+    counts / tau of a circuit, or soft logits), ``scores`` ``[B, beams]`` = each beam's sum of log
+    probabilities (-inf: not in use).  A candidate's score is
+    ``log_softmax(logits)[b, v] + scores[b]`` in 32 bits; equal scores go to the lowest beam,
+    then the lowest token.  A beam with ``finished[b]`` goes on with ``eos`` alone, at its score.
+    Masked logits (-inf or NaN) are chosen only when nothing else is left, with score -inf."""
+    if scores.dim() != 2:
+        raise ValueError(f"beam_step: scores must be [B, beams], got {tuple(scores.shape)}")
+    B, beams = scores.shape
+    if logits.dtype not in DTYPE_ID:
+        raise TypeError(f"beam_step: logits must be float32, bfloat16 or float16, got {logits.dtype}")
+    V = logits.shape[-1]
+    if tuple(logits.shape) not in ((B, beams, V), (B * beams, V)):
+        raise ValueError(f"beam_step: logits {tuple(logits.shape)} do not fit scores {tuple(scores.shape)}")
+    require_cuda(logits, scores, finished)
+    width = beams if width is None else int(width)
+    if not 1 <= beams <= BEAM_MAX or not 1 <= width <= BEAM_MAX:
+        raise ValueError(f"beam_step: beams and width must be in 1..{BEAM_MAX}, got {beams} and {width}")
+    if width > beams * V:
+        raise ValueError(f"beam_step: width {width} exceeds the {beams * V} candidates")
+    if eos is not None and not 0 <= eos < V:
+        raise ValueError(f"beam_step: eos {eos} not in the vocabulary of {V}")
+    if finished is not None:
+        if eos is None:
+            raise ValueError("beam_step: finished needs eos")
+        if finished.shape != scores.shape or finished.dtype not in (torch.bool, torch.uint8):
+            raise ValueError("beam_step: finished must be bool, of the shape of scores")
+        finished = finished.contiguous()
+    dev = logits.device
+    x = logits.reshape(B * beams, V)
+    if B and (x.stride(1) != 1 and V > 1 or x.stride(0) < V):
+        x = x.contiguous()
+    scores = scores.float().contiguous()
+    out = torch.empty((B, width), dtype=torch.float32, device=dev)
+    idx = torch.empty((2, B, width), dtype=torch.int64, device=dev)
+    done = torch.empty((B, width), dtype=torch.bool, device=dev) if eos is not None else None
+    nbytes = lib().slg_beam_step_workspace_bytes(B, beams, V, width)
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+    call("slg_beam_step", ptr(x), DTYPE_ID[x.dtype], B, beams, V, max(x.stride(0), V), ptr(scores),
+         ptr(finished), -1 if eos is None else int(eos), width, ptr(out), ptr(idx[0]), ptr(idx[1]),
+         ptr(done), ptr(ws), nbytes, stream_ptr(dev))
+    return BeamStep(out, idx[0], idx[1], done)
+
+
+@torch.no_grad()
+def beam_reorder(state, parents, layout="rows", beams=None):
+    """The decoder state after a step: sample ``e * width + n`` is the state's sample
+    ``e * beams + parents[e, n]``, for ``parents`` ``[B, width]`` of :func:`beam_step`.
+
+    ``layout``: ``"rows"`` -- ``[B * beams, ...]`` of any type; ``"features"`` -- feature-major
+    fp32 ``[F, ldb]``; ``"packed"`` -- bit-packed ``[F, ldw]`` int64 words, sample s = bit
+    ``s % 64`` of word ``s // 64``.  ``beams`` (default: ``width``; rows: from the shape) is
+    the number of beams that the state holds per entry."""
+    if parents.dim() != 2 or parents.dtype != torch.int64:
+        raise ValueError("beam_reorder: parents must be [B, width] int64")
+    require_cuda(state, parents)
+    B, width = parents.shape
+    parents = parents.contiguous()
+    st = stream_ptr(state.device)
+    state = state.contiguous()
+    if layout == "rows":
+        if beams is None:
+            beams = state.shape[0] // B if B else width
+        if state.dim() < 1 or state.shape[0] != B * beams:
+            raise ValueError(f"beam_reorder: {tuple(state.shape)} does not hold {B} entries of {beams} beams")
+        out = torch.empty((B * width,) + tuple(state.shape[1:]), dtype=state.dtype, device=state.device)
+        nbytes = out[0].numel() * out.element_size() if B else 0
+        call("slg_beam_reorder_rows", ptr(state), nbytes, ptr(parents), B, beams, width, ptr(out), st)
+        return out
+    beams = width if beams is None else int(beams)
+    if layout == "features":
+        want, size, ld_for, fn = torch.float32, 1, _soft.ldb_for, "slg_beam_reorder_features"
+    elif layout == "packed":
+        want, size, ld_for, fn = torch.int64, 64, _hard.ldw_for, "slg_beam_reorder_packed"
+    else:
+        raise ValueError(f"beam_reorder: unknown layout {layout!r}")
+    if state.dim() != 2 or state.dtype != want:
+        raise ValueError(f"beam_reorder: {layout} state must be [F, ld] {want}, got {tuple(state.shape)} {state.dtype}")
+    F, ld = state.shape
+    if beams < 1 or ld * size < B * beams:
+        raise ValueError(f"beam_reorder: rows of {ld} do not hold {B} entries of {beams} beams")
+    out = torch.empty((F, ld if beams == width else ld_for(B * width)), dtype=want, device=state.device)
+    call(fn, ptr(state), F, ld, ptr(parents), B, beams, width, ptr(out), out.shape[1], st)
+    return out

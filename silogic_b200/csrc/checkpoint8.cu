@@ -1,0 +1,159 @@
+// Activation checkpoints in 8 bits.
+//
+// A row of activations is cut into blocks of 128 columns.  A block keeps lo = min and
+// step = (max - lo) / 255 in fp32 and one byte per value:
+//   code = rint((x - lo) * (255 / (max - lo))),   x^ = code * step + lo,   |x - x^| <= step / 2.
+// Every operation is one IEEE rounding (no contraction), so the codes are reproducible by
+// any implementation of these lines.  A block whose step is below 2^-100 is constant
+// (step = 0); a block that holds a value that is not finite reads back as NaN, so it is
+// as visible in the gradients as it would be without checkpoints.
+#include "token_common.cuh"
+
+namespace slg {
+
+constexpr int CK_BLOCK = SLG_CKPT_BLOCK;        // columns per (lo, step)
+constexpr int CK_WARPS = 8;
+constexpr float CK_TINY = 7.888609052210118e-31f;    // 2^-100
+
+static_assert(CK_BLOCK == 128, "a warp handles a block, 4 values per lane");
+
+template <typename T>
+__device__ __forceinline__ void load4(const T* __restrict__ p, int64_t c, int64_t cols, bool vec, float (&v)[4]) {
+    if (vec && c + 4 <= cols) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 q = __ldg(reinterpret_cast<const float4*>(p + c));
+            v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+        } else {
+            union { uint2 u; T e[4]; } q = {__ldg(reinterpret_cast<const uint2*>(p + c))};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = to_f32(q.e[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = c + j < cols ? to_f32(p[c + j]) : 0.0f;
+    }
+}
+
+// one warp = one block of one row
+template <typename T>
+__global__ void __launch_bounds__(CK_WARPS * 32)
+ckpt_store_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t ldx, int vec,
+                  uint32_t* __restrict__ codes, int64_t ldw, float2* __restrict__ bounds, int64_t nblk) {
+    const int lane = threadIdx.x & 31;
+    const int64_t q = (int64_t)blockIdx.x * CK_WARPS + (threadIdx.x >> 5);
+    if (q >= rows * nblk) return;
+    const int64_t row = q / nblk, blk = q - row * nblk;
+    const int64_t c = blk * CK_BLOCK + lane * 4;
+    float v[4];
+    load4(x + row * ldx, c, cols, vec, v);
+    float lo = CUDART_INF_F, hi = -CUDART_INF_F;
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (c + j < cols) {
+            lo = fminf(lo, v[j]);
+            hi = fmaxf(hi, v[j]);
+            bad |= !isfinite(v[j]);
+        }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    const float range = __fsub_rn(hi, lo);
+    bad = __any_sync(0xffffffffu, bad) || !isfinite(range);
+    float step = __fmul_rn(range, 1.0f / 255.0f);
+    const bool flat = bad || step < CK_TINY;
+    const float inv = flat ? 0.0f : __fdiv_rn(255.0f, range);
+    uint32_t word = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (!flat && c + j < cols) {
+            const float code = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(v[j], lo), inv)), 0.0f), 255.0f);
+            word |= (uint32_t)code << (8 * j);
+        }
+    if (c < cols) codes[row * ldw + (c >> 2)] = word;
+    if (lane == 0)
+        bounds[q] = bad ? make_float2(CUDART_NAN_F, CUDART_NAN_F) : make_float2(lo, flat ? 0.0f : step);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(CK_WARPS * 32)
+ckpt_load_kernel(const uint32_t* __restrict__ codes, int64_t ldw, const float2* __restrict__ bounds, int64_t rows,
+                 int64_t cols, int64_t nblk, T* __restrict__ x, int64_t ldx, int vec) {
+    const int lane = threadIdx.x & 31;
+    const int64_t q = (int64_t)blockIdx.x * CK_WARPS + (threadIdx.x >> 5);
+    if (q >= rows * nblk) return;
+    const int64_t row = q / nblk, blk = q - row * nblk;
+    const int64_t c = blk * CK_BLOCK + lane * 4;
+    if (c >= cols) return;
+    const uint32_t word = __ldg(&codes[row * ldw + (c >> 2)]);
+    const float2 b = __ldg(&bounds[q]);
+    union { float4 f; uint2 u; T e[4]; } o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        o.e[j] = from_f32<T>(__fadd_rn(__fmul_rn((float)((word >> (8 * j)) & 255u), b.y), b.x));
+    T* p = x + row * ldx + c;
+    if (vec && c + 4 <= cols) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = o.f;
+        else *reinterpret_cast<uint2*>(p) = o.u;
+    } else {
+        for (int j = 0; j < 4 && c + j < cols; ++j) p[j] = o.e[j];
+    }
+}
+
+static int check_ckpt(const void* codes, int64_t ldc, const void* bounds, int64_t rows, int64_t cols, int64_t ldx,
+                      int dtype, const char* name) {
+    if (rows < 0 || cols < 0) return set_error(SLG_ERR_ARG, "%s: bad sizes", name);
+    if (ldx < cols) return set_error(SLG_ERR_ARG, "%s: ldx < cols", name);
+    if (ldc < cols) return set_error(SLG_ERR_ARG, "%s: ldc < cols", name);
+    if (ldc % 4) return set_error(SLG_ERR_ALIGN, "%s: ldc must be a multiple of 4", name);
+    if (dtype != SLG_DT_F32 && dtype != SLG_DT_BF16 && dtype != SLG_DT_F16)
+        return set_error(SLG_ERR_UNSUPPORTED, "%s: dtype %d not built", name, dtype);
+    if (rows * cols > 0 && (!codes || !bounds)) return set_error(SLG_ERR_ARG, "%s: null pointer", name);
+    if (!aligned_to(codes, 4) || !aligned_to(bounds, 8))
+        return set_error(SLG_ERR_ALIGN, "%s: codes / bounds misaligned", name);
+    if (cdiv(rows * cdiv(cols, CK_BLOCK), CK_WARPS) >= (1ll << 31))
+        return set_error(SLG_ERR_ARG, "%s: too many blocks", name);
+    return SLG_OK;
+}
+
+}  // namespace slg
+
+using namespace slg;
+
+extern "C" int slg_ckpt_store(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ldx, uint8_t* codes,
+                              int64_t ldc, float* bounds, void* stream) {
+    int st = check_ckpt(codes, ldc, bounds, rows, cols, ldx, dtype, "slg_ckpt_store");
+    if (st) return st;
+    if (rows * cols == 0) return SLG_OK;
+    if (!x) return set_error(SLG_ERR_ARG, "slg_ckpt_store: null pointer");
+    const int64_t nblk = cdiv(cols, CK_BLOCK);
+    cudaStream_t s = as_stream(stream);
+    for_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        const int vec = ldx % 4 == 0 && aligned_to(x, 4 * sizeof(T));
+        ckpt_store_kernel<T><<<(unsigned)cdiv(rows * nblk, CK_WARPS), CK_WARPS * 32, 0, s>>>(
+            (const T*)x, rows, cols, ldx, vec, reinterpret_cast<uint32_t*>(codes), ldc / 4,
+            reinterpret_cast<float2*>(bounds), nblk);
+    });
+    return check_launch("slg_ckpt_store");
+}
+
+extern "C" int slg_ckpt_load(const uint8_t* codes, int64_t ldc, const float* bounds, int64_t rows, int64_t cols,
+                             void* x, int32_t dtype, int64_t ldx, void* stream) {
+    int st = check_ckpt(codes, ldc, bounds, rows, cols, ldx, dtype, "slg_ckpt_load");
+    if (st) return st;
+    if (rows * cols == 0) return SLG_OK;
+    if (!x) return set_error(SLG_ERR_ARG, "slg_ckpt_load: null pointer");
+    const int64_t nblk = cdiv(cols, CK_BLOCK);
+    cudaStream_t s = as_stream(stream);
+    for_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        const int vec = ldx % 4 == 0 && aligned_to(x, 4 * sizeof(T));
+        ckpt_load_kernel<T><<<(unsigned)cdiv(rows * nblk, CK_WARPS), CK_WARPS * 32, 0, s>>>(
+            reinterpret_cast<const uint32_t*>(codes), ldc / 4, reinterpret_cast<const float2*>(bounds), rows, cols,
+            nblk, (T*)x, ldx, vec);
+    });
+    return check_launch("slg_ckpt_load");
+}

@@ -1,0 +1,239 @@
+"""Beam selection and state reordering on the GPU against plain 64-bit / integer code.
+
+The selection is checked by value: the scores are within the rounding of their 32-bit
+arithmetic of the 64-bit ones, and the chosen (beam, token) pairs equal the 64-bit choice
+wherever neighbouring candidates lie further apart than that; on logits whose scores are
+exact in 32 bits (zero normaliser spread, integer scores) ties must go to the lowest index.
+"""
+import pytest
+import torch
+
+import silogic_b200 as S
+from silogic_b200 import _hard, _soft
+
+pytestmark = pytest.mark.gpu
+dev = "cuda"
+NEG = -float("inf")
+
+
+def _reference(x, scores, finished, eos, width):
+    """Sorted (value, flat index) of every candidate in 64 bits, best first."""
+    B, k = scores.shape
+    V = x.shape[-1]
+    x = x.double().view(B, k, V).clone()
+    x[torch.isnan(x)] = NEG
+    x = x.clamp(max=torch.finfo(torch.float32).max)
+    m = x.amax(2, keepdim=True)
+    d = torch.where(m > NEG, x - m, NEG)
+    c = d - torch.exp(d).sum(2, keepdim=True).log() + scores.double()[:, :, None]
+    c = torch.where(m > NEG, c, NEG)
+    if finished is not None:
+        only = torch.full_like(c, NEG)
+        only[:, :, eos] = scores.double()
+        c = torch.where(finished[:, :, None], only, c)
+    c = torch.where(torch.isnan(c), NEG, c).view(B, k * V)
+    v, i = torch.sort(c, dim=1, descending=True, stable=True)
+    return c, v[:, :width], i[:, :width]
+
+
+def _check(x, scores, finished=None, eos=None, width=None):
+    r = S.beam_step(x, scores, finished=finished, eos=eos, width=width)
+    B, k = scores.shape
+    V = x.shape[-1]
+    w = width or k
+    c, v, i = _reference(x, scores, finished, eos, w)
+    flat = r.parents * V + r.tokens
+    assert r.scores.shape == (B, w) and r.parents.dtype == torch.int64 and r.tokens.dtype == torch.int64
+    assert bool((r.parents >= 0).all()) and bool((r.parents < k).all())
+    assert bool((r.tokens >= 0).all()) and bool((r.tokens < V).all())
+    # x - m and the logarithm of the sum (V terms in 32 bits) are each rounded, then two sums
+    big = torch.where(torch.isinf(v), 1.0, v.abs()) + scores.abs().where(~torch.isinf(scores), 0).amax(1, keepdim=True)
+    tol = 2.0 ** -22 * (big + 40.0) + V ** 0.5 * 2.0 ** -24
+    same = torch.isinf(v) & (r.scores.double() == v)
+    assert bool((same | ((r.scores.double() - v).abs() <= tol)).all())
+    mine = torch.gather(c, 1, flat)
+    assert bool(((mine == v) | ((mine - v).abs() <= 2 * tol)).all())        # as good as the best
+    gap = torch.full_like(v, 1e30)
+    gap[:, 1:] = torch.minimum(gap[:, 1:], (v[:, :-1] - v[:, 1:]).nan_to_num(0.0))
+    gap[:, :-1] = torch.minimum(gap[:, :-1], (v[:, :-1] - v[:, 1:]).nan_to_num(0.0))
+    sure = (gap > 4 * tol) & ~torch.isinf(v)
+    sure[:, -1] = False                                                     # its successor is not in v
+    assert bool((flat[sure] == i[sure]).all())
+    assert all(len(set(row)) == w for row in flat.tolist())                 # no candidate twice
+    if eos is not None:
+        was = torch.gather(finished, 1, r.parents) if finished is not None else torch.zeros_like(r.finished)
+        assert torch.equal(r.finished, was | (r.tokens == eos))
+    else:
+        assert r.finished is None
+    return r
+
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("B,k,V", [(1, 1, 1), (1, 1, 2), (3, 2, 5), (1, 4, 2000), (5, 3, 1023), (2, 8, 8191), (7, 5, 333),
+                                   (64, 8, 4100), (2, 32, 257), (1, 16, 40001), (300, 2, 64)])
+def test_step_matches_64_bits(B, k, V, dtype):
+    g = torch.Generator().manual_seed(B * 7 + k * 3 + V)
+    x = (4 * torch.randn(B * k, V, generator=g)).to(dtype).to(dev)
+    scores = (-10 * torch.rand(B, k, generator=g)).to(dev)
+    _check(x, scores)
+    if V >= 5:
+        x[torch.rand(B * k, V, generator=g).to(dev) < 0.3] = NEG
+        finished = (torch.rand(B, k, generator=g) < 0.3).to(dev)
+        _check(x.view(B, k, V), scores, finished, eos=V - 1)
+        _check(x, scores, eos=2)
+
+
+@pytest.mark.parametrize("V", [1, 2, 31, 500, 9001])
+def test_ties_go_to_the_lowest_index(V):
+    """Uniform logits: log V is the same for every candidate, so order is by score, beam, token."""
+    k = min(8, V * 2)
+    x = torch.full((2 * k, V), 3.0, device=dev)
+    scores = torch.zeros(2, k, device=dev)
+    scores[1, -1] = 1.0
+    r = S.beam_step(x, scores)
+    want = torch.arange(k, device=dev)
+    assert torch.equal(r.parents[0] * V + r.tokens[0], want)
+    last = [(k - 1) * V + t for t in range(min(V, k))]
+    rest = [i for i in range(k * V) if i not in last][:k - len(last)]
+    assert (r.parents[1] * V + r.tokens[1]).tolist() == (last + rest)[:k]
+
+
+def test_counts_with_many_equal_logits():
+    g = torch.Generator().manual_seed(2)
+    x = (torch.randint(0, 4, (4, 3000), generator=g).float() / 10).to(dev)
+    scores = torch.tensor([[0.0, -30.0, -60.0, -90.0]], device=dev)
+    r = S.beam_step(x, scores)
+    top = torch.nonzero(x[0] == x[0].max()).flatten()[:4]          # the first beam's largest count
+    assert r.parents.tolist() == [[0, 0, 0, 0]] and torch.equal(r.tokens[0], top)
+
+
+def test_masked_rows_and_values_that_are_not_finite():
+    k, V = 4, 600
+    x = torch.randn(2 * k, V, device=dev)
+    x[0] = NEG                                        # a beam with nothing left
+    x[1] = float("nan")
+    x[2, 100:] = float("nan")
+    x[3] = torch.finfo(torch.float32).min             # masked with the type's lowest value
+    x[4:] = NEG                                       # an entry with nothing left
+    scores = torch.tensor([[0.0, 0.0, -1.0, -50.0], [0.0, -1.0, -2.0, -3.0]], device=dev)
+    r = _check(x, scores)
+    assert bool((r.parents[0] == 2).all()) and bool((r.tokens[0] < 100).all())
+    assert r.scores[1].tolist() == [NEG] * 4 and (r.parents[1] * V + r.tokens[1]).tolist() == [0, 1, 2, 3]
+    x[2] = NEG
+    r = S.beam_step(x, scores)                        # only the lowest-value row is left: uniform
+    assert bool((r.parents[0] == 3).all()) and r.tokens[0].tolist() == [0, 1, 2, 3]
+    assert (r.scores[0].double() + 50.0 + torch.log(torch.tensor(600.0)).item()).abs().max() < 1e-4
+    x[0, 7] = float("inf")                            # counts as the largest finite value
+    r = S.beam_step(x, scores)
+    assert (r.parents[0, 0].item(), r.tokens[0, 0].item(), r.scores[0, 0].item()) == (0, 7, 0.0)
+
+
+def test_beams_that_are_not_in_use_and_all_finished():
+    x = torch.randn(4, 50, device=dev)
+    scores = torch.tensor([[0.0, NEG, NEG, NEG]], device=dev)
+    r = _check(x, scores)
+    assert bool((r.parents == 0).all())
+    done = torch.ones(1, 4, dtype=torch.bool, device=dev)
+    scores = torch.tensor([[-4.0, -1.0, -3.0, -2.0]], device=dev)
+    r = S.beam_step(x, scores, finished=done, eos=9)
+    assert r.parents.tolist() == [[1, 3, 2, 0]] and bool((r.tokens == 9).all()) and bool(r.finished.all())
+    assert r.scores.tolist() == [[-1.0, -2.0, -3.0, -4.0]]
+
+
+@pytest.mark.parametrize("k,width", [(1, 4), (1, 32), (4, 2), (3, 7), (32, 1)])
+def test_width_other_than_the_number_of_beams(k, width):
+    g = torch.Generator().manual_seed(k)
+    x = torch.randn(5 * k, 777, generator=g).to(dev)
+    _check(x, -torch.rand(5, k, generator=g).to(dev), width=width)
+
+
+def test_strided_logits_and_fewer_tokens_than_beams():
+    base = torch.randn(6, 1000, device=dev)
+    scores = torch.zeros(2, 3, device=dev)
+    for x in (base[:, 3:503], base[:, ::2], base[:, 1:4].t().contiguous().t(), base[:1].expand(6, 1000)):
+        a, b = S.beam_step(x, scores), S.beam_step(x.contiguous(), scores)
+        assert torch.equal(a.scores, b.scores) and torch.equal(a.parents, b.parents) and torch.equal(a.tokens, b.tokens)
+    _check(torch.randn(8, 2, device=dev), torch.zeros(1, 8, device=dev))
+
+
+def _src(parents, beams):
+    B = parents.shape[0]
+    return (torch.arange(B, device=dev)[:, None] * beams + parents).reshape(-1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.uint8, torch.int64, torch.bool])
+@pytest.mark.parametrize("shape", [(), (1,), (3,), (7, 5), (64,), (1000,)])
+@pytest.mark.parametrize("B,k,w", [(1, 1, 1), (3, 4, 4), (5, 2, 6), (65, 8, 8)])
+def test_reorder_rows(B, k, w, shape, dtype):
+    g = torch.Generator().manual_seed(B + k)
+    state = torch.randint(0, 200, (B * k,) + shape, generator=g).to(dtype).to(dev)
+    parents = torch.randint(0, k, (B, w), generator=g).to(dev)
+    got = S.beam_reorder(state, parents)
+    assert got.dtype == dtype and torch.equal(got, state[_src(parents, k)])
+
+
+@pytest.mark.parametrize("F", [1, 3, 100, 2001])
+@pytest.mark.parametrize("B,k,w", [(1, 1, 1), (1, 4, 4), (3, 5, 5), (16, 8, 8), (9, 32, 32), (5, 2, 6), (64, 8, 3)])
+def test_reorder_features_and_packed(F, B, k, w):
+    g = torch.Generator().manual_seed(F + B + k)
+    parents = torch.randint(0, k, (B, w), generator=g).to(dev)
+    src = _src(parents, k)
+    x = torch.rand(B * k, F, generator=g).to(dev)
+    xt = torch.zeros(F, _soft.ldb_for(B * k), device=dev)
+    xt[:, :B * k] = x.t()
+    got = S.beam_reorder(xt, parents, layout="features", beams=k)
+    assert got.shape == (F, _soft.ldb_for(B * w) if w != k else xt.shape[1])
+    assert torch.equal(got[:, :B * w], xt[:, src]) and bool((got[:, B * w:] == 0).all())
+    bits = (x > 0.5).to(torch.uint8)
+    packed = _hard.pack(bits)
+    got = S.beam_reorder(packed, parents, layout="packed", beams=k)
+    assert torch.equal(_hard.unpack(got, B * w), bits[src])
+    assert torch.equal(got, _hard.pack(bits[src].contiguous(), ldw=got.shape[1]))       # padding bits 0
+
+
+def test_reorder_keeps_a_wider_row_and_takes_strided_state():
+    bits = (torch.rand(10, 33, device=dev) > 0.5).to(torch.uint8)
+    packed = _hard.pack(bits, ldw=6)
+    parents = torch.tensor([[4, 0, 0, 2, 1], [3, 3, 3, 4, 0]], device=dev)
+    got = S.beam_reorder(packed, parents, layout="packed")
+    assert got.shape == packed.shape and torch.equal(got, _hard.pack(bits[_src(parents, 5)].contiguous(), ldw=6))
+    state = torch.rand(8, 10, 3, device=dev).transpose(0, 1)
+    assert torch.equal(S.beam_reorder(state, parents), state[_src(parents, 5)])
+
+
+def test_empty_batches():
+    r = S.beam_step(torch.empty(0, 50, device=dev), torch.empty(0, 4, device=dev), eos=3)
+    assert r.scores.shape == (0, 4) and r.finished.shape == (0, 4)
+    p = torch.empty(0, 4, dtype=torch.int64, device=dev)
+    assert S.beam_reorder(torch.empty(0, 7, device=dev), p).shape == (0, 7)
+    assert S.beam_reorder(torch.empty(5, 4, device=dev), p, layout="features").shape == (5, 4)
+    one = torch.zeros(1, 4, dtype=torch.int64, device=dev)
+    assert S.beam_reorder(torch.empty(4, 0, device=dev), one).shape == (4, 0)
+    assert S.beam_reorder(torch.empty(0, 4, device=dev), one, layout="features").shape == (0, 4)
+
+
+def test_step_on_another_stream_and_in_a_graph():
+    x, scores = torch.randn(8, 900, device=dev), torch.zeros(2, 4, device=dev)
+    state = torch.rand(8, 33, device=dev)
+
+    def both():
+        r = S.beam_step(x, scores, eos=3)
+        return r.scores, r.parents, r.tokens, r.finished, S.beam_reorder(state, r.parents)
+    want = both()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = both()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(want, other))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = both()
+    for seed in range(3):
+        torch.manual_seed(seed)
+        x.normal_()
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(kept, both()))

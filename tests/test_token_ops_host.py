@@ -1,0 +1,101 @@
+"""Refusals of the token, checkpoint and beam entry points (no GPU needed: arguments are
+checked before anything is launched)."""
+import ctypes
+import os
+
+import pytest
+import torch
+
+import silogic_b200 as S
+from silogic_b200 import _lib
+
+
+@pytest.fixture(scope="module")
+def L():
+    if not os.path.exists(_lib.LIB_PATH):
+        from silogic_b200 import build
+        build.build()
+    return _lib.lib()
+
+
+def _p(v):
+    return ctypes.c_void_p(v)
+
+
+def test_python_entry_points_refuse_wrong_arguments():
+    w, ids = torch.randn(10, 4), torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(TypeError, match="weight"):
+        S.token_embedding(ids, w.double())
+    with pytest.raises(TypeError, match="weight"):
+        S.token_embedding(ids, w[0])
+    with pytest.raises(TypeError, match="ids"):
+        S.token_embedding(ids.float(), w)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        S.token_embedding(ids, w)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        S.checkpoint8_store(w)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        S.beam_step(torch.randn(4, 10), torch.zeros(2, 2))
+    with pytest.raises(ValueError, match="scores"):
+        S.beam_step(torch.randn(4, 10), torch.zeros(4))
+    with pytest.raises(ValueError, match="do not fit"):
+        S.beam_step(torch.randn(5, 10), torch.zeros(2, 2))
+    with pytest.raises(TypeError, match="logits"):
+        S.beam_step(torch.zeros(4, 10, dtype=torch.int64), torch.zeros(2, 2))
+    with pytest.raises(ValueError, match="parents"):
+        S.beam_reorder(torch.randn(4, 10), torch.zeros(2, 2))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        S.beam_reorder(torch.randn(4, 10), torch.zeros(2, 2, dtype=torch.int64))
+
+
+def test_checkpoint8_switch_nests_and_resets_on_errors():
+    from silogic_b200 import _soft
+    assert _soft.CHECKPOINT8 is False
+    with pytest.raises(KeyError):
+        with S.checkpoint8():
+            assert _soft.CHECKPOINT8 is True
+            with S.checkpoint8(False):
+                assert _soft.CHECKPOINT8 is False
+            assert _soft.CHECKPOINT8 is True
+            raise KeyError
+    assert _soft.CHECKPOINT8 is False
+
+
+def test_c_entry_points_refuse_bad_arguments(L):
+    # embedding: sizes, types, null pointers, alignment, workspace
+    fwd = lambda **k: L.slg_embed_fwd(_p(k.get("ids", 256)), k.get("i64", 1), k.get("N", 4), _p(256),       # noqa: E731
+                                      k.get("dt", 0), k.get("V", 10), k.get("D", 8), 1.0, _p(k.get("out", 256)), _p(0))
+    assert fwd(N=-1) == 1 and fwd(V=0) == 1 and fwd(D=0) == 1 and fwd(i64=2) == 1
+    assert fwd(dt=3) == 3 and fwd(N=1 << 31) == 3 and fwd(V=(1 << 31) - 1) == 3
+    assert fwd(ids=0) == 1 and fwd(out=260) == 2 and b"aligned" in L.slg_last_error()
+    assert fwd(N=0, ids=0) == 0                                            # nothing to do
+    need = L.slg_embed_bwd_workspace_bytes(100, 10, 8, 0)
+    assert need > 0 and L.slg_embed_bwd_workspace_bytes(-1, 10, 8, 0) == 0
+    bwd = lambda n=100, gw=256, ws=256, size=need, dt=0: L.slg_embed_bwd(                                  # noqa: E731
+        _p(256), 1, n, _p(256), dt, 10, 8, 1.0, -1, _p(gw), _p(ws), size, _p(0))
+    assert bwd(size=need - 1) == 5 and bwd(gw=0) == 1 and bwd(ws=0) == 1 and bwd(ws=264) == 2
+    assert bwd(n=-1) == 1 and bwd(dt=7) == 3
+    # checkpoints
+    store = lambda x=256, rows=4, cols=10, ldx=10, codes=256, ldc=12, bounds=256, dt=0: L.slg_ckpt_store(  # noqa: E731
+        _p(x), dt, rows, cols, ldx, _p(codes), ldc, _p(bounds), _p(0))
+    assert store(rows=-1) == 1 and store(ldx=9) == 1 and store(ldc=8) == 1 and store(ldc=11) == 2
+    assert store(dt=9) == 3 and store(codes=0) == 1 and store(x=0) == 1 and store(codes=258) == 2 and store(bounds=260) == 2
+    assert store(rows=0, codes=0, bounds=0, x=0) == 0
+    load = lambda x=256, rows=4, cols=10, ldx=10, codes=256, ldc=12, bounds=256, dt=0: L.slg_ckpt_load(    # noqa: E731
+        _p(codes), ldc, _p(bounds), rows, cols, _p(x), dt, ldx, _p(0))
+    assert load(cols=-1) == 1 and load(ldc=11) == 2 and load(dt=-1) == 3 and load(x=0) == 1
+    # beams
+    need = L.slg_beam_step_workspace_bytes(2, 4, 50, 4)
+    step = lambda B=2, k=4, V=50, ldx=50, w=4, dt=0, fin=0, eos=-1, x=256, size=need: L.slg_beam_step(     # noqa: E731
+        _p(x), dt, B, k, V, ldx, _p(256), _p(fin), eos, w, _p(256), _p(256), _p(256), _p(0), _p(256), size, _p(0))
+    assert step(B=-1) == 1 and step(V=0) == 1 and step(ldx=49) == 1 and step(k=33, size=1 << 20) == 3
+    assert step(w=33, size=1 << 20) == 3 and step(k=1, V=2, ldx=2, w=3) == 1 and step(dt=5) == 3
+    assert step(fin=256, eos=-1) == 1 and step(fin=256, eos=50) == 1 and step(x=0) == 1
+    assert step(B=0, x=0) == 0
+    if need:
+        assert step(size=need - 1) == 5
+    rows = lambda i=256, o=512, nb=16, B=2: L.slg_beam_reorder_rows(_p(i), nb, _p(256), B, 4, 4, _p(o), _p(0))   # noqa: E731
+    assert rows(i=0) == 1 and rows(o=256) == 1 and rows(nb=-1) == 1 and rows(B=0) == 0 and rows(nb=0) == 0
+    assert L.slg_beam_reorder_features(_p(256), 3, 7, _p(256), 2, 4, 4, _p(512), 8, _p(0)) == 1       # rows too short
+    assert L.slg_beam_reorder_features(_p(256), 3, 8, _p(256), 2, 4, 4, _p(512), 7, _p(0)) == 1
+    assert L.slg_beam_reorder_packed(_p(256), 3, 1, _p(256), 20, 4, 4, _p(512), 2, _p(0)) == 1

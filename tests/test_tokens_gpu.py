@@ -1,0 +1,178 @@
+"""Token embedding on the GPU against a plain 64-bit implementation.
+
+Tolerances: the lookup rounds scale * w once in 32 bits and once to the type
+(u = 2^-24, 2^-8, 2^-11 for fp32, bf16, fp16 as the spacing bound of one rounding); a
+gradient row of n terms is summed in 32 bits, (n + 2) 2^-24 of the sum of magnitudes, and
+rounded once.
+"""
+import pytest
+import torch
+
+import silogic_b200 as S
+
+pytestmark = pytest.mark.gpu
+dev = "cuda"
+UNIT = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+SMALLEST = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+NAMES = ["fp32", "bf16", "fp16"]
+
+
+def _case(V, D, N, dtype, seed=0, ids=None, idt=torch.int64):
+    g = torch.Generator().manual_seed(seed)
+    w = torch.randn(V, D, generator=g).to(dtype).to(dev)
+    if ids is None:     # frequencies fall as 1 / rank: a few tokens fill most of the batch
+        ids = (torch.exp(torch.rand(N, generator=g) * torch.log(torch.tensor(V + 1.0))).long() - 1).clamp(0, V - 1)
+    gy = torch.randn(len(ids), D, generator=g).to(dtype).to(dev)
+    return ids.to(idt).to(dev), w, gy
+
+
+def _check_grad(got, ids, gy, V, scale, pad=None):
+    ids, g64 = ids.reshape(-1).long(), gy.reshape(ids.numel(), gy.shape[-1]).double()
+    keep = (ids >= 0) & (ids < V)
+    if pad is not None:
+        keep &= ids != pad
+    want = torch.zeros(V, g64.shape[1], dtype=torch.float64, device=dev).index_add_(0, ids[keep], g64[keep])
+    mag = torch.zeros_like(want).index_add_(0, ids[keep], g64[keep].abs())
+    n = torch.bincount(ids[keep], minlength=V).double()[:, None]
+    u = UNIT[got.dtype]
+    tol = abs(scale) * mag * (n + 2) * 2.0 ** -24 + (abs(scale) * want.abs()) * u + SMALLEST[got.dtype]
+    err = (got.double() - scale * want).abs()
+    assert got.shape == want.shape and bool((err <= tol).all()), f"worst excess {(err - tol).max().item():.3e}"
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+@pytest.mark.parametrize("V,D,N", [(1, 1, 1), (7, 3, 5), (50, 64, 33), (256, 128, 257), (255, 331, 1021),
+                                   (10000, 784, 4), (1000, 100, 20000), (65536, 40, 3000), (65537, 8, 70001),
+                                   (300, 1030, 513)])
+def test_lookup_and_gradient_match_64_bits(V, D, N, dtype):
+    ids, w, gy = _case(V, D, N, dtype, seed=V + D + N, idt=torch.int32 if N % 2 else torch.int64)
+    w.requires_grad_(True)
+    scale = D ** 0.5
+    y = S.token_embedding(ids, w, scale=scale)
+    assert y.dtype == dtype and y.shape == (N, D)
+    want = w.detach().double()[ids.long()] * scale
+    tol = want.abs() * (UNIT[dtype] + 2.0 ** -23) + SMALLEST[dtype]
+    assert bool(((y.double() - want).abs() <= tol).all())
+    (gw,) = torch.autograd.grad(y, w, gy)
+    assert gw.dtype == dtype
+    _check_grad(gw, ids, gy, V, scale)
+
+
+@pytest.mark.parametrize("N", [0, 1, 31, 4096, 4097, 9000, 300000])
+def test_gradient_of_one_hot_token_and_empty_batch(N):
+    """Every token the same: one row takes the whole sum, the others are zero."""
+    ids, w, gy = _case(37, 20, N, torch.float32, ids=torch.full((N,), 5))
+    w.requires_grad_(True)
+    y = S.token_embedding(ids, w, scale=0.5)
+    (gw,) = torch.autograd.grad(y, w, gy)
+    _check_grad(gw, ids, gy, 37, 0.5)
+    assert bool((gw[:5] == 0).all()) and bool((gw[6:] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+@pytest.mark.parametrize("D", [64, 65])
+def test_padding_and_out_of_range_ids(D, dtype):
+    V, N = 100, 5000
+    g = torch.Generator().manual_seed(3)
+    raw = torch.randint(-3, V + 3, (N,), generator=g)
+    ids, w, gy = _case(V, D, N, dtype, ids=raw)
+    w.requires_grad_(True)
+    y = S.token_embedding(ids, w, padding_idx=7)
+    bad = (ids < 0) | (ids >= V)
+    assert bool(torch.isnan(y[bad]).all()) and not bool(torch.isnan(y[~bad]).any())
+    assert torch.equal(y[ids == 7], w.detach()[7].expand(int((ids == 7).sum()), D))   # read like any row
+    (gw,) = torch.autograd.grad(y, w, gy)
+    _check_grad(gw, ids, gy, V, 1.0, pad=7)
+    assert bool((gw[7] == 0).all())
+    with pytest.raises(IndexError):
+        S.token_embedding(ids, w, check=True)
+
+
+def test_ids_of_any_shape_strided_weights_and_gradients():
+    base = torch.randn(60, 48, device=dev)
+    w = base[::2, ::3].requires_grad_(True)                  # not contiguous
+    ids = torch.randint(0, 30, (4, 5, 6), device=dev).transpose(0, 2)
+    y = S.token_embedding(ids, w, scale=2.0)
+    assert y.shape == (6, 5, 4, 16) and torch.equal(y, 2.0 * w.detach()[ids])
+    gy = torch.randn(16, 4, 5, 6, device=dev).permute(3, 2, 1, 0)
+    (gw,) = torch.autograd.grad(y, w, gy)
+    _check_grad(gw, ids, gy.contiguous(), 30, 2.0)
+    one = torch.ones((), device=dev).expand(6, 5, 4, 16)     # a broadcast upstream gradient
+    (gw,) = torch.autograd.grad(S.token_embedding(ids, w), w, one)
+    _check_grad(gw, ids, one.contiguous(), 30, 1.0)
+
+
+def test_rows_that_start_on_no_vector_boundary():
+    flat = torch.randn(1 + 50 * 64, device=dev)
+    w = flat[1:].view(50, 64)                                # 4 bytes past a 16-byte boundary
+    ids = torch.randint(0, 50, (333,), device=dev)
+    assert torch.equal(S.token_embedding(ids, w), w[ids])
+    gflat = torch.randn(1 + 333 * 64, device=dev)
+    gy = gflat[1:].view(333, 64)
+    w2 = w.clone().requires_grad_(True)
+    (gw,) = torch.autograd.grad(S.token_embedding(ids, w2), w2, gy)
+    _check_grad(gw, ids, gy, 50, 1.0)
+
+
+def test_gradient_is_the_same_from_run_to_run_and_on_another_stream():
+    ids, w, gy = _case(2000, 256, 50000, torch.float32)
+    w.requires_grad_(True)
+
+    def grad():
+        return torch.autograd.grad(S.token_embedding(ids, w), w, gy)[0]
+    first = grad()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = grad()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(first, other) and torch.equal(first, grad())
+
+
+def test_gradient_against_differences():
+    """dL/dW of L = sum(c * y^2): the directional derivative equals the difference quotient
+    of the (quadratic) loss, which a central difference gives without truncation error."""
+    V, D, N = 40, 24, 300
+    ids, w, c = _case(V, D, N, torch.float32, seed=5)
+    w.requires_grad_(True)
+    loss = lambda m: (c.double() * S.token_embedding(ids, m, scale=1.5).double() ** 2).sum()   # noqa: E731
+    (gw,) = torch.autograd.grad(loss(w), w)
+    d = torch.randn(V, D, generator=torch.Generator().manual_seed(1)).to(dev)
+    h = 2.0 ** -6
+    with torch.no_grad():
+        num = (loss(w + h * d) - loss(w - h * d)) / (2 * h)
+    # the terms of both losses, rounded to 32 bits, divided by 2 h; the gradient's own rounding
+    scale = (c.abs().double() * (1.5 * (w.detach().abs() + h * d.abs()))[ids].double() ** 2).sum()
+    tol = 8 * 2.0 ** -24 * scale / (2 * h)
+    assert abs(num - (gw.double() * d.double()).sum()) <= tol
+
+
+def test_inside_a_cuda_graph():
+    ids, w, gy = _case(500, 96, 777, torch.float32)
+    w.requires_grad_(True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(S.token_embedding(ids, w), w, gy)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = S.token_embedding(ids, w)
+        (gw,) = torch.autograd.grad(y, w, gy)
+    for seed in (1, 2):
+        new, _, _ = _case(500, 96, 777, torch.float32, seed=seed)
+        ids.copy_(new)
+        graph.replay()
+        assert torch.equal(y, w.detach()[ids])
+        _check_grad(gw, ids, gy, 500, 1.0)
+
+
+def test_module_trains_and_keeps_its_padding_row():
+    torch.manual_seed(0)
+    m = S.TokenEmbedding(50, 16, padding_idx=3).to(dev)
+    assert bool((m.weight[3] == 0).all()) and m.scale == 4.0
+    ids = torch.randint(0, 50, (8, 9), device=dev)
+    ids[0] = 3
+    m(ids).sum().backward()
+    assert bool((m.weight.grad[3] == 0).all()) and bool((m.weight.grad != 0).any())
