@@ -386,6 +386,19 @@ int slg_ckpt_store(const void* x, int32_t dtype, int64_t rows, int64_t cols, int
 int slg_ckpt_load(const uint8_t* codes, int64_t ldc, const float* bounds, int64_t rows,
                   int64_t cols, void* x, int32_t dtype, int64_t ldx, void* stream);
 
+/* slg_fc_soft_bwd with the layer's input read from an 8-bit checkpoint of its
+ * feature-major activations: codes [in_dim, ldc], bounds [in_dim,
+ * ceil(ldb / SLG_CKPT_BLOCK), 2]; the other arguments and the workspace are those of
+ * slg_fc_soft_bwd.  Built for the (K, node, arity) that _built() answers with 1; for the
+ * others restore the activations (slg_ckpt_load) and call slg_fc_soft_bwd. */
+int32_t slg_fc_soft_bwd_ckpt_built(int32_t K, int32_t node, int32_t arity);
+int slg_fc_soft_bwd_ckpt(const uint8_t* codes, int64_t ldc, const float* bounds, int64_t in_dim,
+                         int64_t ldb, const int32_t* cand, const float* conn, int32_t K,
+                         int32_t conn_ste, int32_t node, int32_t arity, const float* params,
+                         int32_t gate_hard, float inv_tau, int64_t out_dim, int64_t wire_r,
+                         const float* gy, float* gx, float* gconn, float* gparams,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+
 /* One step of beam search.  logits [B * beams, V] with row stride ldx, scores [B, beams]
  * (sums of log probabilities so far; -inf for a beam that is not in use).  Candidate
  * (b, v) has (x - max_b) - log(sum exp(x - max_b)) + scores[b]; a beam with finished[b]
@@ -393,13 +406,12 @@ int slg_ckpt_load(const uint8_t* codes, int64_t ldc, const float* bounds, int64_
  * out in order, equal values by the lowest b * V + v: their values, beams (parents), tokens and,
  * when out_finished is given, finished[parent] || token == eos.  NaN logits count as
  * masked (-inf), +inf as the largest finite value; masked candidates (value -inf) come
- * last.  beams, width <= SLG_BEAM_MAX; finished and out_finished may be NULL. */
+ * last.  beams, width <= SLG_BEAM_MAX, V < 2^27; finished and out_finished may be NULL. */
 #define SLG_BEAM_MAX 32
-int64_t slg_beam_step_workspace_bytes(int64_t B, int32_t beams, int64_t V, int32_t width);
 int slg_beam_step(const void* logits, int32_t dtype, int64_t B, int32_t beams, int64_t V,
                   int64_t ldx, const float* scores, const uint8_t* finished, int32_t eos,
                   int32_t width, float* out_scores, int64_t* parents, int64_t* tokens,
-                  uint8_t* out_finished, void* workspace, int64_t workspace_bytes, void* stream);
+                  uint8_t* out_finished, void* stream);
 
 /* Decoder state after a step: sample r = e * width + n of `out` is sample
  * e * beams + parents[e, n] of `in` (a parent outside [0, beams) reads beam 0).

@@ -60,8 +60,9 @@ _SIGS = {
     "slg_embed_bwd": [_p, _i32, _i64, _p, _i32, _i64, _i64, _f32, _i64, _p, _p, _i64, _p],
     "slg_ckpt_store": [_p, _i32, _i64, _i64, _i64, _p, _i64, _p, _p],
     "slg_ckpt_load": [_p, _i64, _p, _i64, _i64, _p, _i32, _i64, _p],
-    "slg_beam_step": [_p, _i32, _i64, _i32, _i64, _i64, _p, _p, _i32, _i32, _p, _p, _p, _p, _p,
-                      _i64, _p],
+    "slg_fc_soft_bwd_ckpt": [_p, _i64, _p, _i64, _i64, _p, _p, _i32, _i32, _i32, _i32, _p, _i32,
+                             _f32, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p],
+    "slg_beam_step": [_p, _i32, _i64, _i32, _i64, _i64, _p, _p, _i32, _i32, _p, _p, _p, _p, _p],
     "slg_beam_reorder_rows": [_p, _i64, _p, _i64, _i32, _i32, _p, _p],
     "slg_beam_reorder_features": [_p, _i64, _i64, _p, _i64, _i32, _i32, _p, _i64, _p],
     "slg_beam_reorder_packed": [_p, _i64, _i64, _p, _i64, _i32, _i32, _p, _i64, _p],
@@ -72,8 +73,8 @@ _RESTYPES = {
     "slg_fc_soft_workspace_bytes": ([_i64, _i32, _i32, _i32, _i64], ctypes.c_int64),
     "slg_conv_soft_workspace_bytes": ([_i64, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
                                        _i64], ctypes.c_int64),
+    "slg_fc_soft_bwd_ckpt_built": ([_i32, _i32, _i32], _i32),
     "slg_embed_bwd_workspace_bytes": ([_i64, _i64, _i64, _i32], ctypes.c_int64),
-    "slg_beam_step_workspace_bytes": ([_i64, _i32, _i64, _i32], ctypes.c_int64),
 }
 
 _lib = None
@@ -138,9 +139,15 @@ def call(name, *args):
         raise SilogicError(f"{name} failed with status {st}: {msg}")
 
 
+# the handle without building a torch Stream object (a few microseconds a launch)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_ptr(device=None):
     """Raw handle of torch's current CUDA stream on ``device``."""
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    if _raw_stream is not None and device is not None and device.index is not None:
+        return _raw_stream(device.index)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def ptr(t):

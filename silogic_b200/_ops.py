@@ -373,6 +373,19 @@ def fc_soft_bwd_ckpt(codes: Tensor, bounds: Tensor, ldb: int, cand: Tensor, conn
                      inv_tau: float, out_dim: int, wire_r: int, gy: Tensor,
                      need_gx: bool) -> Tuple[Tensor, Tensor, Tensor]:
     """:func:`fc_soft_bwd` at the activations that an 8-bit checkpoint stands for."""
+    if lib().slg_fc_soft_bwd_ckpt_built(K, node, arity):
+        gy = gy.contiguous()
+        gx = gy.new_zeros((codes.shape[0], ldb)) if need_gx else None
+        gparams = torch.empty_like(params)
+        gconn = torch.empty_like(conn) if conn is not None else None
+        nbytes = lib().slg_fc_soft_workspace_bytes(ldb, K, node, arity, out_dim)
+        ws = torch.empty(max(nbytes, 4) // 4 + 1, dtype=torch.float32, device=gy.device)
+        call("slg_fc_soft_bwd_ckpt", ptr(codes), codes.shape[1], ptr(bounds), codes.shape[0], ldb,
+             ptr(cand), ptr(conn), K, ste, node, arity, ptr(params), gate_hard, inv_tau, out_dim,
+             wire_r, ptr(gy), ptr(gx), ptr(gconn), ptr(gparams), ptr(ws), ws.numel() * 4,
+             stream_ptr(gy.device))
+        return (gx if gx is not None else _empty(gy.device), gparams,
+                gconn if gconn is not None else _empty(gy.device))
     xt = IMPL["ckpt_load"](codes, bounds, ldb, torch.float32)
     return IMPL["fc_soft_bwd"](xt, cand, conn, params, K, ste, node, arity, gate_hard, inv_tau, out_dim,
                        wire_r, gy, need_gx)

@@ -30,6 +30,11 @@ def _keep_checkpoint(ctx):
     return CHECKPOINT8 and any(ctx.needs_input_grad[:3])
 
 
+def _store(xt, meta):
+    """Codes and bounds of the samples' columns (padding columns must not widen a block)."""
+    return op("ckpt_store")(xt[:, :meta.get("batch") or xt.shape[1]])
+
+
 # ------------------------------------------------------------- transposes
 class ToFeatureMajor(torch.autograd.Function):
     @staticmethod
@@ -117,7 +122,7 @@ class FCSoft(torch.autograd.Function):
         y = op("fc_soft_fwd")(xt, meta["cand"], connc, params, *FCSoft._args(meta))
         ctx.ckpt = _keep_checkpoint(ctx)
         if ctx.ckpt:        # the backward pass works from 8-bit codes; xt itself is let go
-            ctx.save_for_backward(*op("ckpt_store")(xt), params, connc)
+            ctx.save_for_backward(*_store(xt, meta), params, connc)
             ctx.ldb = xt.shape[1]
         else:
             ctx.save_for_backward(xt, params, connc)
@@ -140,8 +145,10 @@ class FCSoft(torch.autograd.Function):
                 gconn if connc is not None else None, None)
 
 
-def fc_layer_fm(layer, xt, wire_r=0):
+def fc_layer_fm(layer, xt, wire_r=0, batch=None):
+    """``batch``: samples in ``xt`` (default: every column is one)."""
     meta, params, conn = _fc_meta(layer, wire_r)
+    meta["batch"] = batch
     return FCSoft.apply(xt, params, conn, meta)
 
 
@@ -149,7 +156,7 @@ def logic_layer_forward(layer, x):
     """``LogicLayer.forward`` on ``[B, in]``."""
     require_cuda(x)
     B = x.shape[0]
-    return FromFeatureMajor.apply(fc_layer_fm(layer, ToFeatureMajor.apply(x)), B)
+    return FromFeatureMajor.apply(fc_layer_fm(layer, ToFeatureMajor.apply(x), batch=B), B)
 
 
 def node_forward(node, x, idx):
@@ -162,7 +169,7 @@ def node_forward(node, x, idx):
     fake = SimpleNamespace(node=node, _conn=conn, arity=node.arity, out_dim=node.out_dim,
                            in_dim=x.reshape(x.shape[0], -1).shape[1], training=node.training)
     meta, params, c = _fc_meta(fake)
-    B = x.shape[0]
+    B = meta["batch"] = x.shape[0]
     return FromFeatureMajor.apply(FCSoft.apply(ToFeatureMajor.apply(x), params, c, meta), B)
 
 
@@ -194,7 +201,7 @@ def logic_net_features_fm(net, x):
     xt = ToFeatureMajor.apply(x)
     for layer in net.layers:
         wr = net.wire_r if (net.wire_r and layer.in_dim == layer.out_dim) else 0
-        xt = fc_layer_fm(layer, xt, wr)
+        xt = fc_layer_fm(layer, xt, wr, B)
     return xt, B
 
 
@@ -290,7 +297,7 @@ class ConvSoft(torch.autograd.Function):
                                    keep)
         ctx.ckpt = _keep_checkpoint(ctx)
         if ctx.ckpt:
-            ctx.save_for_backward(*op("ckpt_store")(xt), params, connc, arg)
+            ctx.save_for_backward(*_store(xt, meta), params, connc, arg)
             ctx.ldb = xt.shape[1]
         else:
             ctx.save_for_backward(xt, params, connc, arg)
@@ -367,9 +374,10 @@ def conv_soft_bwd_deterministic(xt, shape, m, params, connc, gy):
     return gx, gparams, gconn
 
 
-def conv_block_fm(conv, xt, shape, wire_r=0, pool=1):
+def conv_block_fm(conv, xt, shape, wire_r=0, pool=1, batch=None):
     """One conv block on feature-major ``xt`` ([C*H*W, ldb]); returns (yt, (n, Hp, Wp))."""
     meta, params, conn = _conv_meta(conv, wire_r, pool)
+    meta["batch"] = batch
     C, H, W = shape
     Ho = H + 2 * conv.padding - conv.kh + 1
     Wo = W + 2 * conv.padding - conv.kw + 1
@@ -385,9 +393,9 @@ def logic_conv_net_features_fm(net, x):
     for i in range(0, len(blocks), 2):
         conv, pool = blocks[i], blocks[i + 1]
         assert isinstance(pool, OrPool)
-        xt, shape = conv_block_fm(conv, xt, shape, net.wire_channels(conv, shape[0]), pool.size)
+        xt, shape = conv_block_fm(conv, xt, shape, net.wire_channels(conv, shape[0]), pool.size, B)
     for layer in net.head_layers:
-        xt = fc_layer_fm(layer, xt)
+        xt = fc_layer_fm(layer, xt, batch=B)
     return xt, B
 
 
@@ -408,7 +416,7 @@ def conv_tree_forward(conv, x, pool=1):
     """``ConvLogicTree.forward`` on ``[B, C, H, W]`` -> ``[B, n, Ho, Wo]``."""
     require_cuda(x)
     B, C, H, W = x.shape
-    yt, (n, Hp, Wp) = conv_block_fm(conv, ToFeatureMajor.apply(x), (C, H, W), 0, pool)
+    yt, (n, Hp, Wp) = conv_block_fm(conv, ToFeatureMajor.apply(x), (C, H, W), 0, pool, B)
     return FromFeatureMajor.apply(yt, B).view(B, n, Hp, Wp)
 
 

@@ -6,7 +6,7 @@ from collections import namedtuple
 import torch
 
 from . import _hard, _soft
-from ._lib import call, lib, ptr, require_cuda, stream_ptr
+from ._lib import call, ptr, require_cuda, stream_ptr
 from ._ops import DTYPE_ID
 
 BEAM_MAX = 32           # SLG_BEAM_MAX
@@ -31,7 +31,9 @@ def beam_step(logits, scores, finished=None, eos=None, width=None):
     B, beams = scores.shape
     if logits.dtype not in DTYPE_ID:
         raise TypeError(f"beam_step: logits must be float32, bfloat16 or float16, got {logits.dtype}")
-    V = logits.shape[-1]
+    V = logits.shape[-1] if logits.dim() else 0
+    if V >= 1 << 27:
+        raise ValueError(f"beam_step: vocabulary of {V} (must be below 2**27)")
     if tuple(logits.shape) not in ((B, beams, V), (B * beams, V)):
         raise ValueError(f"beam_step: logits {tuple(logits.shape)} do not fit scores {tuple(scores.shape)}")
     require_cuda(logits, scores, finished)
@@ -54,14 +56,13 @@ def beam_step(logits, scores, finished=None, eos=None, width=None):
         x = x.contiguous()
     scores = scores.float().contiguous()
     out = torch.empty((B, width), dtype=torch.float32, device=dev)
-    idx = torch.empty((2, B, width), dtype=torch.int64, device=dev)
+    parents = torch.empty((B, width), dtype=torch.int64, device=dev)
+    tokens = torch.empty((B, width), dtype=torch.int64, device=dev)
     done = torch.empty((B, width), dtype=torch.bool, device=dev) if eos is not None else None
-    nbytes = lib().slg_beam_step_workspace_bytes(B, beams, V, width)
-    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-    call("slg_beam_step", ptr(x), DTYPE_ID[x.dtype], B, beams, V, max(x.stride(0), V), ptr(scores),
-         ptr(finished), -1 if eos is None else int(eos), width, ptr(out), ptr(idx[0]), ptr(idx[1]),
-         ptr(done), ptr(ws), nbytes, stream_ptr(dev))
-    return BeamStep(out, idx[0], idx[1], done)
+    call("slg_beam_step", x.data_ptr(), DTYPE_ID[x.dtype], B, beams, V, max(x.stride(0), V), scores.data_ptr(),
+         ptr(finished), -1 if eos is None else int(eos), width, out.data_ptr(), parents.data_ptr(),
+         tokens.data_ptr(), ptr(done), stream_ptr(dev))
+    return BeamStep(out, parents, tokens, done)
 
 
 @torch.no_grad()

@@ -6,124 +6,273 @@
 // finished beam has the one candidate (b, eos) at its own score.  Masked logits (-inf, or
 // NaN) are never chosen while another candidate is left; +inf counts as the largest finite
 // value.  (x - m) - log s keeps rows apart whose logits are huge or at the type's lowest value.
+#include <cooperative_groups.h>
+#include <utility>
+
 #include "token_common.cuh"
+
 
 namespace slg {
 
-constexpr int BM_THREADS = 256;
+namespace cg = cooperative_groups;
+
+constexpr int BM_THREADS = 512;
 constexpr int BM_WARPS = BM_THREADS / 32;
+constexpr int BM_PER = 32;              // logits a lane holds at once
+constexpr int BM_UNIT = 32 * BM_PER;    // logits of one unit of a warp's work
 constexpr int BM_MAX = SLG_BEAM_MAX;
 constexpr float BM_LARGEST = 3.402823466e+38f;
 
-// candidate order: larger value first, then the lower index
-__device__ __forceinline__ bool ahead(float v, int64_t i, float w, int64_t j) { return v > w || (v == w && i < j); }
+// NaN -> -inf, +inf -> the largest finite value (fmaxf returns its other argument for NaN)
+__device__ __forceinline__ float clean(float v) { return fminf(fmaxf(v, -CUDART_INF_F), BM_LARGEST); }
 
-__device__ __forceinline__ float clean(float v) { return v != v ? -CUDART_INF_F : fminf(v, BM_LARGEST); }
-
-struct Cand { float v; int32_t i; };
-constexpr int32_t NO_INDEX = 0x7fffffff;
-
-__device__ __forceinline__ Cand warp_best(Cand c) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float v = __shfl_xor_sync(0xffffffffu, c.v, o);
-        const int32_t i = __shfl_xor_sync(0xffffffffu, c.i, o);
-        if (ahead(v, i, c.v, c.i)) { c.v = v; c.i = i; }
-    }
-    return c;
+// Candidate order as one integer: larger value first, then the lower index.  0 = none.
+__device__ __forceinline__ uint32_t ordered(float v) {
+    const uint32_t u = __float_as_uint(v + 0.0f);           // -0 -> +0
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(uint32_t o) {
+    return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ uint64_t cand_key(float v, uint32_t index) {
+    return ((uint64_t)ordered(v) << 32) | (uint32_t)~index;
+}
+__device__ __forceinline__ uint64_t warp_max(uint64_t k) {
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32));
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+    return ((uint64_t)hi << 32) | lo;
 }
 
-// One CTA = one beam: its `width` best tokens, in order.
+// The n largest keys of mem[0 .. count), keys being distinct; lane i returns the i-th
+// (0: there is none).
+__device__ __forceinline__ uint64_t warp_select(const uint64_t* mem, int count, int n, int lane) {
+    uint64_t last = ~0ull, mine = 0;
+    for (int i = 0; i < n; ++i) {
+        uint64_t k = 0;
+        for (int c = lane; c < count; c += 32) {
+            const uint64_t v = mem[c];
+            if (v < last && v > k) k = v;
+        }
+        last = warp_max(k);
+        if (lane == i) mine = last;
+        if (last == 0) break;
+    }
+    return mine;
+}
+
+// One cluster = one entry.  A beam's logits are cut into units of 1,024, its units into
+// `parts` runs, and every warp of the cluster takes (beam, part) items.  Of an item a warp
+// keeps, in one pass, each lane's running maximum and sum of exponentials, and the `width`
+// largest logits (lane i: the i-th): a unit is only searched while one of its lanes' maxima
+// beats the list's last, so later units cost little more than their loads.  It leaves (max,
+// sum, list) in the first CTA's shared memory; that CTA joins maxima and sums per beam,
+// turns lists into scores, and selects.  Which lane sums which logits depends on their place in
+// the row alone: beams with the same logits get the same normaliser, and tie.
+struct BeamSlots {
+    uint64_t* key;          // [items][width] (ordered logit, ~token); then (ordered score, ~index)
+    float* m;               // [items]
+    float* s;               // [items]
+};
+
+__host__ __device__ inline int beam_parts(int cs, int beams, int units) {
+    const int p = cs * BM_WARPS / beams;
+    return p < 1 ? 1 : p < units ? p : units;
+}
+// at most 39 KB (8 CTAs, 32 beams, width 32)
+static inline size_t beam_smem(int items, int beams, int width) {
+    return (size_t)items * (width * 8 + 8) + (size_t)BM_WARPS * width * 8 + beams * 8;
+}
+
+// logits [at, at + E) of a row of V, masked past its end
 template <typename T>
-__global__ void __launch_bounds__(BM_THREADS)
-beam_row_kernel(const T* __restrict__ x, int64_t V, int64_t ldx, const float* __restrict__ scores,
-                const uint8_t* __restrict__ finished, int32_t eos, int width, float* __restrict__ val,
-                int32_t* __restrict__ tok) {
-    __shared__ float red[BM_WARPS];
-    __shared__ Cand best[BM_WARPS];
+__device__ __forceinline__ void load_logits(const T* __restrict__ row, bool aligned, int64_t at, int64_t V, float* x,
+                                            uint32_t& valid, int bit) {
+    constexpr int E = Pack16<T>::E;
+    if (aligned && at + E <= V) {
+        unpack16<T>(__ldg(reinterpret_cast<const uint4*>(row + at)), x);
+#pragma unroll
+        for (int j = 0; j < E; ++j) x[j] = clean(x[j]);
+        valid |= ((1u << E) - 1u) << bit;
+    } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const bool on = at + j < V;
+            x[j] = on ? clean(to_f32(row[at + j])) : -CUDART_INF_F;
+            valid |= (on ? 1u : 0u) << (bit + j);
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(BM_THREADS, 2)
+beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams, int units, const float* __restrict__ scores,
+                 const uint8_t* __restrict__ finished, int32_t eos, int width, float* __restrict__ out_scores,
+                 int64_t* __restrict__ parents, int64_t* __restrict__ tokens, uint8_t* __restrict__ out_finished) {
+    constexpr int E = Pack16<T>::E;
+    extern __shared__ uint64_t smem[];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int cs = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t row = blockIdx.x;
-    const T* p = x + row * ldx;
-    const float S = scores[row];
-    const bool done = finished && finished[row];
-    float m = -CUDART_INF_F, logs = 0.0f;
-    if (!done) {
-        for (int64_t v = threadIdx.x; v < V; v += BM_THREADS) m = fmaxf(m, clean(to_f32(p[v])));
+    const int64_t entry = blockIdx.x / cs;
+    const int parts = beam_parts(cs, beams, units), items = beams * parts;
+    BeamSlots own;
+    own.key = smem;
+    uint64_t* best = own.key + (size_t)items * width;               // [warps][width]
+    own.m = reinterpret_cast<float*>(best + BM_WARPS * width);
+    own.s = own.m + items;
+    float* beam_m = own.s + items;                                  // [beams] maximum, log of the sum
+    float* beam_l = beam_m + beams;
+
+    auto started = cluster.barrier_arrive();                        // the first CTA's memory is there
+    bool waited = false;
+    for (int item = rank * BM_WARPS + warp; item < items; item += cs * BM_WARPS) {
+        const int b = item / parts, part = item - b * parts;
+        const int64_t row_at = entry * beams + b;
+        const bool done = finished && finished[row_at];
+        uint64_t list = 0;                                          // lane i: the i-th best so far
+        float m = -CUDART_INF_F, s = 0.0f;
+        if (done) {
+            // eos at the beam's own score, the other tokens masked: the first part lists them
+            const int t = lane == 0 ? eos : lane - 1 + (lane - 1 >= eos);
+            if (part == 0 && lane < width && t < V) list = cand_key(lane == 0 ? 0.0f : -CUDART_INF_F, (uint32_t)t);
+        } else {
+            const T* row = logits + row_at * ldx;
+            const bool aligned = (reinterpret_cast<uintptr_t>(row) & 15u) == 0;
+            const int q1 = (int)((int64_t)units * (part + 1) / parts);
+            for (int q = (int)((int64_t)units * part / parts); q < q1; ++q) {
+                const int64_t base = (int64_t)q * BM_UNIT + lane * E;
+                float x[BM_PER];
+                uint32_t valid = 0;
+#pragma unroll
+                for (int j = 0; j < BM_PER / E; ++j)
+                    load_logits<T>(row, aligned, base + j * 32 * E, V, x + j * E, valid, j * E);
+                float top = x[0];
+#pragma unroll
+                for (int i = 1; i < BM_PER; ++i) top = fmaxf(top, x[i]);
+                if (top > m) {
+                    s *= __expf(m - top);                           // exp(-inf) = 0 at the start
+                    m = top;
+                }
+                const float ref = m > -CUDART_INF_F ? m : 0.0f;
+#pragma unroll
+                for (int i = 0; i < BM_PER; ++i) s += __expf(x[i] - ref);
+                // search: the lane's best untaken logit, its lowest index first
+                uint32_t left = valid;
+                uint64_t k = 0;
+                auto next = [&]() {
+                    float v = -CUDART_INF_F;
+                    int at = -1;
+#pragma unroll
+                    for (int i = 0; i < BM_PER; ++i)
+                        if ((left >> i & 1u) && (at < 0 || x[i] > v)) { v = x[i]; at = i; }
+                    k = at < 0 ? 0 : cand_key(v, (uint32_t)(base + (at / E) * 32 * E + at % E));
+                    if (at >= 0) left &= ~(1u << at);
+                };
+                uint64_t bar = __shfl_sync(0xffffffffu, list, width - 1);
+                if (!__any_sync(0xffffffffu, valid && ordered(top) >= (uint32_t)(bar >> 32))) continue;
+                next();
+                for (;;) {
+                    const uint64_t w = warp_max(k);
+                    if (w <= bar) break;                            // also when nothing is left (0)
+                    if (k == w) next();
+                    const int at = __popc(__ballot_sync(0xffffffffu, lane < width && list > w));
+                    const uint64_t up = __shfl_up_sync(0xffffffffu, list, 1);
+                    if (lane < width && lane >= at) list = lane == at ? w : up;
+                    bar = __shfl_sync(0xffffffffu, list, width - 1);
+                }
+            }
+        }
+        // lanes' maxima and sums -> the warp's
+        float mw = m;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mw = fmaxf(mw, __shfl_xor_sync(0xffffffffu, mw, o));
+        float sw = m > -CUDART_INF_F ? s * __expf(m - mw) : 0.0f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sw += __shfl_xor_sync(0xffffffffu, sw, o);
+        if (!waited) {
+            cluster.barrier_wait(std::move(started));
+            waited = true;
+        }
+        uint64_t* key0 = cluster.map_shared_rank(own.key, 0);
+        if (lane < width) key0[(size_t)item * width + lane] = list;
+        if (lane == 0) {
+            *cluster.map_shared_rank(own.m + item, 0) = mw;
+            *cluster.map_shared_rank(own.s + item, 0) = sw;
+        }
+    }
+    if (!waited) cluster.barrier_wait(std::move(started));
+    cluster.sync();
+    if (rank != 0) return;
+
+    for (int b = warp; b < beams; b += BM_WARPS) {
+        float m = -CUDART_INF_F;
+        for (int i = b * parts + lane; i < (b + 1) * parts; i += 32) m = fmaxf(m, own.m[i]);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (lane == 0) red[warp] = m;
-        __syncthreads();
-        for (int q = 0; q < BM_WARPS; ++q) m = fmaxf(m, red[q]);
-        __syncthreads();
         float s = 0.0f;
-        if (m > -CUDART_INF_F)
-            for (int64_t v = threadIdx.x; v < V; v += BM_THREADS) s += expf(clean(to_f32(p[v])) - m);
+        for (int i = b * parts + lane; i < (b + 1) * parts; i += 32)
+            if (own.m[i] > -CUDART_INF_F) s += own.s[i] * expf(own.m[i] - m);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) red[warp] = s;
-        __syncthreads();
-        s = 0.0f;
-        for (int q = 0; q < BM_WARPS; ++q) s += red[q];
-        logs = logf(s);
+        if (lane == 0) { beam_m[b] = m; beam_l[b] = logf(s); }
     }
-    auto value = [&](int64_t v) {
-        float l = -CUDART_INF_F;
-        if (done) l = v == eos ? S : l;
-        else if (m > -CUDART_INF_F) l = (clean(to_f32(p[v])) - m) - logs + S;
-        return l != l ? -CUDART_INF_F : l;
-    };
-    Cand last = {CUDART_INF_F, -1};
-    for (int n = 0; n < width; ++n) {
-        Cand c = {-CUDART_INF_F, NO_INDEX};
-        for (int64_t v = threadIdx.x; v < V; v += BM_THREADS) {
-            const float l = value(v);
-            if (ahead(last.v, last.i, l, v) && ahead(l, v, c.v, c.i)) c = {l, (int32_t)v};
+    __syncthreads();
+    // logits -> scores, in place; the index of (beam, token) is beam V + token
+    for (int i = threadIdx.x; i < items * width; i += BM_THREADS) {
+        const int b = i / (width * parts);
+        const uint64_t k = own.key[i];
+        uint64_t r = 0;
+        if (k != 0) {
+            const float S = scores[entry * beams + b], x = unordered((uint32_t)(k >> 32));
+            const bool done = finished && finished[entry * beams + b];
+            float v = done ? x + S : beam_m[b] > -CUDART_INF_F ? (x - beam_m[b]) - beam_l[b] + S : -CUDART_INF_F;
+            if (v != v) v = -CUDART_INF_F;
+            r = cand_key(v, (uint32_t)b * (uint32_t)V + ~(uint32_t)k);
         }
-        c = warp_best(c);
-        __syncthreads();
-        if (lane == 0) best[warp] = c;
-        __syncthreads();
-        for (int q = 0; q < BM_WARPS; ++q)
-            if (ahead(best[q].v, best[q].i, c.v, c.i)) c = best[q];
-        last = c;
-        if (threadIdx.x == 0) { val[row * width + n] = c.v; tok[row * width + n] = c.i; }
+        own.key[i] = r;
+    }
+    __syncthreads();
+    {   // each warp its run of items, then one warp the warps' winners
+        const int a = items * warp / BM_WARPS, e = items * (warp + 1) / BM_WARPS;
+        const uint64_t k = warp_select(own.key + (size_t)a * width, (e - a) * width, width, lane);
+        if (lane < width) best[warp * width + lane] = k;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        const uint64_t k = warp_select(best, BM_WARPS * width, width, lane);
+        if (lane < width) {
+            const uint32_t at = ~(uint32_t)k;
+            const int b = (int)(at / (uint32_t)V);
+            const int64_t t = at - (uint32_t)b * (uint32_t)V, o = entry * width + lane;
+            out_scores[o] = unordered((uint32_t)(k >> 32));
+            parents[o] = b;
+            tokens[o] = t;
+            if (out_finished) out_finished[o] = (finished && finished[entry * beams + b]) || t == eos;
+        }
     }
 }
 
-// One warp = one entry: the best of its beams' lists, which are in order.
-__global__ void beam_join_kernel(const float* __restrict__ val, const int32_t* __restrict__ tok, int64_t B, int beams,
-                                 int64_t V, int width, const uint8_t* __restrict__ finished, int32_t eos,
-                                 float* __restrict__ scores, int64_t* __restrict__ parents,
-                                 int64_t* __restrict__ tokens, uint8_t* __restrict__ done) {
-    const int lane = threadIdx.x & 31;
-    const int64_t b = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    if (b >= B) return;
-    int at = 0;                                             // lane = beam: its next candidate
-    for (int n = 0; n < width; ++n) {
-        float v = -CUDART_INF_F;
-        int64_t i = INT64_MAX;
-        if (lane < beams && at < width) {
-            const int64_t q = ((int64_t)b * beams + lane) * width + at;
-            v = val[q];
-            if (tok[q] != NO_INDEX) i = lane * V + tok[q];
-        }
-        float bv = v;
-        int64_t bi = i;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
-            const int64_t oi = __shfl_xor_sync(0xffffffffu, bi, o);
-            if (ahead(ov, oi, bv, bi)) { bv = ov; bi = oi; }
-        }
-        if (bi == i && i != INT64_MAX) {
-            ++at;
-            const int64_t t = i - lane * V;
-            scores[b * width + n] = v;
-            parents[b * width + n] = lane;
-            tokens[b * width + n] = t;
-            if (done) done[b * width + n] = (finished && finished[b * beams + lane]) || t == eos;
-        }
-    }
+template <typename T>
+static cudaError_t beam_step_launch(const T* x, int64_t B, int beams, int64_t V, int64_t ldx, const float* scores,
+                                    const uint8_t* finished, int32_t eos, int width, float* out_scores, int64_t* parents,
+                                    int64_t* tokens, uint8_t* out_finished, cudaStream_t st) {
+    const int units = (int)cdiv(V, BM_UNIT);
+    // CTAs per entry: as many as have a unit for every warp, at most 8, no more than fill the GPU
+    int cs = 1;
+    while (cs < 8 && (int64_t)cs * BM_WARPS < (int64_t)beams * units && B * cs < 2 * sm_count()) cs *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(B * cs));
+    cfg.blockDim = dim3(BM_THREADS);
+    cfg.dynamicSmemBytes = beam_smem(beams * beam_parts(cs, beams, units), beams, width);
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = cs;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, beam_step_kernel<T>, x, V, ldx, beams, units, scores, finished, eos, width, out_scores,
+                              parents, tokens, out_finished);
 }
 
 // ----------------------------------------------------------------- reorder
@@ -177,44 +326,31 @@ __global__ void reorder_packed_kernel(const uint32_t* __restrict__ in, int64_t F
 
 using namespace slg;
 
-extern "C" int64_t slg_beam_step_workspace_bytes(int64_t B, int32_t beams, int64_t V, int32_t width) {
-    (void)V;
-    if (B <= 0 || beams <= 0 || width <= 0) return 0;
-    return B * beams * width * 8;
-}
-
 extern "C" int slg_beam_step(const void* logits, int32_t dtype, int64_t B, int32_t beams, int64_t V, int64_t ldx,
                              const float* scores, const uint8_t* finished, int32_t eos, int32_t width,
                              float* out_scores, int64_t* parents, int64_t* tokens, uint8_t* out_finished,
-                             void* workspace, int64_t workspace_bytes, void* stream) {
+                             void* stream) {
     const char* name = "slg_beam_step";
     if (B < 0 || beams <= 0 || V <= 0 || width <= 0) return set_error(SLG_ERR_ARG, "%s: bad sizes", name);
     if (beams > BM_MAX || width > BM_MAX)
         return set_error(SLG_ERR_UNSUPPORTED, "%s: at most %d beams", name, BM_MAX);
-    if (V >= (1ll << 31) - 1) return set_error(SLG_ERR_UNSUPPORTED, "%s: vocabulary must be below 2^31 - 1", name);
+    if (V >= 1 << 27) return set_error(SLG_ERR_UNSUPPORTED, "%s: vocabulary must be below 2^27", name);
     if (width > beams * V) return set_error(SLG_ERR_ARG, "%s: width %d > beams * vocabulary", name, width);
     if (ldx < V) return set_error(SLG_ERR_ARG, "%s: ldx < vocabulary", name);
     if (finished && (eos < 0 || eos >= V)) return set_error(SLG_ERR_ARG, "%s: finished needs eos in the vocabulary", name);
     if (dtype != SLG_DT_F32 && dtype != SLG_DT_BF16 && dtype != SLG_DT_F16)
         return set_error(SLG_ERR_UNSUPPORTED, "%s: dtype %d not built", name, dtype);
-    if (B * beams >= (1ll << 31)) return set_error(SLG_ERR_ARG, "%s: batch too large", name);
+    if (B >= 1 << 27) return set_error(SLG_ERR_ARG, "%s: batch too large", name);
     if (B == 0) return SLG_OK;
-    if (!logits || !scores || !out_scores || !parents || !tokens || !workspace)
+    if (!logits || !scores || !out_scores || !parents || !tokens)
         return set_error(SLG_ERR_ARG, "%s: null pointer", name);
-    const int64_t need = slg_beam_step_workspace_bytes(B, beams, V, width);
-    if (workspace_bytes < need)
-        return set_error(SLG_ERR_WORKSPACE, "%s: workspace %lld < %lld bytes", name, (long long)workspace_bytes,
-                         (long long)need);
-    cudaStream_t s = as_stream(stream);
-    float* val = static_cast<float*>(workspace);
-    int32_t* tok = reinterpret_cast<int32_t*>(val + B * beams * width);
+    cudaError_t e = cudaSuccess;
     for_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        beam_row_kernel<T><<<(unsigned)(B * beams), BM_THREADS, 0, s>>>((const T*)logits, V, ldx, scores, finished,
-                                                                       eos, width, val, tok);
+        e = beam_step_launch<T>((const T*)logits, B, beams, V, ldx, scores, finished, eos, width, out_scores, parents,
+                                tokens, out_finished, as_stream(stream));
     });
-    beam_join_kernel<<<(unsigned)cdiv(B, 4), 128, 0, s>>>(val, tok, B, beams, V, width, finished, eos, out_scores,
-                                                          parents, tokens, out_finished);
+    if (e != cudaSuccess) return set_error(SLG_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
     return check_launch(name);
 }
 

@@ -24,9 +24,9 @@ __device__ __forceinline__ void load4(const T* __restrict__ p, int64_t c, int64_
             const float4 q = __ldg(reinterpret_cast<const float4*>(p + c));
             v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
         } else {
-            union { uint2 u; T e[4]; } q = {__ldg(reinterpret_cast<const uint2*>(p + c))};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = to_f32(q.e[j]);
+            const uint2 q = __ldg(reinterpret_cast<const uint2*>(p + c));
+            unpack2<T>(q.x, v);
+            unpack2<T>(q.y, v + 2);
         }
     } else {
 #pragma unroll
@@ -89,16 +89,17 @@ ckpt_load_kernel(const uint32_t* __restrict__ codes, int64_t ldw, const float2* 
     if (c >= cols) return;
     const uint32_t word = __ldg(&codes[row * ldw + (c >> 2)]);
     const float2 b = __ldg(&bounds[q]);
-    union { float4 f; uint2 u; T e[4]; } o;
+    float v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        o.e[j] = from_f32<T>(__fadd_rn(__fmul_rn((float)((word >> (8 * j)) & 255u), b.y), b.x));
+    for (int j = 0; j < 4; ++j) v[j] = __fadd_rn(__fmul_rn((float)((word >> (8 * j)) & 255u), b.y), b.x);
     T* p = x + row * ldx + c;
     if (vec && c + 4 <= cols) {
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = o.f;
-        else *reinterpret_cast<uint2*>(p) = o.u;
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        else *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(v), pack2<T>(v + 2));
     } else {
-        for (int j = 0; j < 4 && c + j < cols; ++j) p[j] = o.e[j];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c + j < cols) p[j] = from_f32<T>(v[j]);
     }
 }
 

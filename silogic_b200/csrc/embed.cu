@@ -19,40 +19,35 @@ template <typename T, typename I, bool VEC>
 __global__ void __launch_bounds__(EM_THREADS)
 embed_fwd_kernel(const I* __restrict__ ids, int64_t N, const T* __restrict__ w, int64_t V, int64_t D,
                  float scale, T* __restrict__ y) {
-    constexpr int E = Vec16<T>::E;
+    constexpr int E = Pack16<T>::E;
     const int64_t total = N * D;
     const int64_t base = ((int64_t)blockIdx.x * EM_THREADS * EM_UNROLL + threadIdx.x) * E;
-    Vec16<T> v[EM_UNROLL];
 #pragma unroll
     for (int u = 0; u < EM_UNROLL; ++u) {
         const int64_t e0 = base + (int64_t)u * EM_THREADS * E;
         if (e0 >= total) continue;
+        int64_t i = e0 / D, c = e0 - i * D;
+        int64_t t = (int64_t)ids[i];
+        float v[E];
         if constexpr (VEC) {
-            const int64_t i = e0 / D, c = e0 - i * D;
-            const int64_t t = (int64_t)ids[i];
-            if (t >= 0 && t < V) v[u].u = __ldg(reinterpret_cast<const uint4*>(w + t * D + c));
+            if (t >= 0 && t < V) unpack16<T>(__ldg(reinterpret_cast<const uint4*>(w + t * D + c)), v);
             else
 #pragma unroll
-                for (int j = 0; j < E; ++j) v[u].e[j] = from_f32<T>(CUDART_NAN_F);
+                for (int j = 0; j < E; ++j) v[j] = CUDART_NAN_F;
         } else {
-            int64_t i = e0 / D, c = e0 - i * D;
-            int64_t t = (int64_t)ids[i];
 #pragma unroll
             for (int j = 0; j < E; ++j) {
-                if (e0 + j < total) v[u].e[j] = t >= 0 && t < V ? w[t * D + c] : from_f32<T>(CUDART_NAN_F);
+                v[j] = e0 + j >= total ? 0.0f : t >= 0 && t < V ? to_f32(w[t * D + c]) : CUDART_NAN_F;
                 if (++c == D && e0 + j + 1 < total) { c = 0; t = (int64_t)ids[++i]; }
             }
         }
-    }
 #pragma unroll
-    for (int u = 0; u < EM_UNROLL; ++u) {
-        const int64_t e0 = base + (int64_t)u * EM_THREADS * E;
-        if (e0 >= total) continue;
-#pragma unroll
-        for (int j = 0; j < E; ++j) v[u].e[j] = from_f32<T>(to_f32(v[u].e[j]) * scale);
-        if (e0 + E <= total) *reinterpret_cast<uint4*>(y + e0) = v[u].u;
+        for (int j = 0; j < E; ++j) v[j] *= scale;
+        if (e0 + E <= total) *reinterpret_cast<uint4*>(y + e0) = pack16<T>(v);
         else
-            for (int j = 0; e0 + j < total; ++j) y[e0 + j] = v[u].e[j];
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                if (e0 + j < total) y[e0 + j] = from_f32<T>(v[j]);
     }
 }
 
@@ -197,33 +192,48 @@ __device__ __forceinline__ Cut merge_cut(const uint32_t* __restrict__ key, int64
     return {lo, d - lo};
 }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_cols(const T* __restrict__ row, int64_t c0, int64_t D, int lane,
-                                          Vec16<T>& v) {
-    constexpr int E = Vec16<T>::E;
-    if constexpr (VEC) {
+// A lane's E values of columns [c0, c0 + 32 E) of a row: one vector, or (VEC false: rows
+// start on no 16-byte boundary) every 32nd value.
+template <typename T, bool VEC> struct Cols {
+    static constexpr int E = Pack16<T>::E;
+    uint4 u;
+    __device__ __forceinline__ void load(const T* __restrict__ row, int64_t c0, int64_t D, int lane) {
         const int64_t c = c0 + lane * E;
-        if (c < D) v.u = __ldg(reinterpret_cast<const uint4*>(row + c));
-        else v.u = make_uint4(0, 0, 0, 0);
-    } else {
+        u = c < D ? __ldg(reinterpret_cast<const uint4*>(row + c)) : make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void add_to(float (&acc)[E]) const {
+        float x[E];
+        unpack16<T>(u, x);
+#pragma unroll
+        for (int j = 0; j < E; ++j) acc[j] += x[j];
+    }
+};
+template <typename T> struct Cols<T, false> {
+    static constexpr int E = Pack16<T>::E;
+    T x[E];
+    __device__ __forceinline__ void load(const T* __restrict__ row, int64_t c0, int64_t D, int lane) {
 #pragma unroll
         for (int j = 0; j < E; ++j) {
             const int64_t c = c0 + lane + 32 * j;
-            v.e[j] = c < D ? row[c] : from_f32<T>(0.0f);
+            x[j] = c < D ? row[c] : from_f32<T>(0.0f);
         }
     }
-}
+    __device__ __forceinline__ void add_to(float (&acc)[E]) const {
+#pragma unroll
+        for (int j = 0; j < E; ++j) acc[j] += to_f32(x[j]);
+    }
+};
 
 template <typename T, bool VEC>
 __device__ __forceinline__ void store_row(T* __restrict__ row, int64_t c0, int64_t D, int lane, float scale,
-                                          const float (&acc)[Vec16<T>::E]) {
-    constexpr int E = Vec16<T>::E;
+                                          const float (&acc)[Pack16<T>::E]) {
+    constexpr int E = Pack16<T>::E;
     if constexpr (VEC) {
         const int64_t c = c0 + lane * E;
-        Vec16<T> v;
+        float v[E];
 #pragma unroll
-        for (int j = 0; j < E; ++j) v.e[j] = from_f32<T>(acc[j] * scale);
-        if (c < D) *reinterpret_cast<uint4*>(row + c) = v.u;
+        for (int j = 0; j < E; ++j) v[j] = acc[j] * scale;
+        if (c < D) *reinterpret_cast<uint4*>(row + c) = pack16<T>(v);
     } else {
 #pragma unroll
         for (int j = 0; j < E; ++j) {
@@ -258,7 +268,7 @@ __global__ void __launch_bounds__(SG_WARPS * 32)
 embed_sum_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ pos, int64_t N, int64_t V,
                  int64_t D, int64_t chunk, const T* __restrict__ g, float scale, T* __restrict__ gw,
                  float* __restrict__ carry, int64_t slices, int32_t* __restrict__ head_row) {
-    constexpr int E = Vec16<T>::E;
+    constexpr int E = Pack16<T>::E;
     constexpr int SLICE = 32 * E;
     __shared__ Cut cut[2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -294,19 +304,18 @@ embed_sum_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ 
             }
         };
         for (int64_t i = i0; i < i1; i += SG_UNROLL) {
-            Vec16<T> v[SG_UNROLL];
+            Cols<T, VEC> v[SG_UNROLL];
             uint32_t k[SG_UNROLL];
 #pragma unroll
             for (int u = 0; u < SG_UNROLL; ++u) {
                 k[u] = i + u < i1 ? key[i + u] : 0u;
-                if (i + u < i1) load_cols<T, VEC>(g + (int64_t)pos[i + u] * D, c0, D, lane, v[u]);
+                if (i + u < i1) v[u].load(g + (int64_t)pos[i + u] * D, c0, D, lane);
             }
 #pragma unroll
             for (int u = 0; u < SG_UNROLL; ++u) {
                 if (i + u >= i1) break;
                 end_rows((int64_t)k[u]);
-#pragma unroll
-                for (int j = 0; j < E; ++j) acc[j] += to_f32(v[u].e[j]);
+                v[u].add_to(acc);
             }
         }
         end_rows(r1);
@@ -320,7 +329,7 @@ __global__ void __launch_bounds__(SG_WARPS * 32)
 embed_join_kernel(const uint32_t* __restrict__ key, int64_t N, int64_t V, int64_t D, int64_t chunk,
                   int64_t nchunk, float scale, T* __restrict__ gw, const float* __restrict__ carry,
                   int64_t slices, const int32_t* __restrict__ head_row) {
-    constexpr int E = Vec16<T>::E;
+    constexpr int E = Pack16<T>::E;
     constexpr int SLICE = 32 * E;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t c = blockIdx.x;
@@ -386,9 +395,9 @@ static int check_embed(int64_t N, int64_t V, int64_t D, int ids64, int dtype, co
 template <typename T, typename I>
 static void embed_fwd_launch(const I* ids, int64_t N, const T* w, int64_t V, int64_t D, float scale, T* y,
                              cudaStream_t st) {
-    const int64_t vecs = cdiv(N * D, Vec16<T>::E);
+    const int64_t vecs = cdiv(N * D, Pack16<T>::E);
     const unsigned grid = (unsigned)cdiv(vecs, EM_THREADS * EM_UNROLL);
-    if (D % Vec16<T>::E == 0 && aligned16(w))
+    if (D % Pack16<T>::E == 0 && aligned16(w))
         embed_fwd_kernel<T, I, true><<<grid, EM_THREADS, 0, st>>>(ids, N, w, V, D, scale, y);
     else
         embed_fwd_kernel<T, I, false><<<grid, EM_THREADS, 0, st>>>(ids, N, w, V, D, scale, y);
@@ -434,7 +443,7 @@ static void embed_bwd_launch(const uint32_t* key, int64_t N, int64_t V, int64_t 
             embed_join_kernel<T, VEC><<<grid, SG_WARPS * 32, 0, st>>>(key, N, V, D, p.chunk, p.nchunk, scale, gw,
                                                                       carry, p.slices, head);
     };
-    if (D % Vec16<T>::E == 0 && aligned16(g) && aligned16(gw)) go(std::true_type{});
+    if (D % Pack16<T>::E == 0 && aligned16(g) && aligned16(gw)) go(std::true_type{});
     else go(std::false_type{});
 }
 

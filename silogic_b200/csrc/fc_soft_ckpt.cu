@@ -1,0 +1,216 @@
+// Backward of a soft FC layer whose input was kept as an 8-bit checkpoint
+// (checkpoint8.cu): fc_soft_bwd_kernel with the gathers reading codes.
+//
+// A warp owns a node and walks 512 samples, 128 at a time -- one block of each candidate
+// row, so (lo, step) are warp-uniform.  With q the codes, x = step q + lo:
+//   a_j   = sum_k w_jk x_jk = sum_k (w_jk step_jk) q_jk + sum_k w_jk lo_jk
+//   dL/dw_jk = sum_b ga_j x_jk = step_jk sum_b ga_j q_jk + lo_jk sum_b ga_j
+// so the codes are used as they are and the bounds enter once per block.  A gather moves 1
+// byte instead of 4, and the node's 16 code words (4 samples each) stay in registers
+// between the two uses.  Partials, their finish kernel and the vector atomics of gx are the
+// fp32 kernel's.
+#include "fc_soft_impl.cuh"
+
+namespace slg {
+
+// byte j of a code word as a float: 2^23 + q has q in its low mantissa bits
+__device__ __forceinline__ float code_f32(uint32_t word, int j) {
+    return __uint_as_float(__byte_perm(word, 0x4b000000u, 0x7540u + j)) - 8388608.0f;
+}
+// twice byte j, from 2^24 + 2 q: another expression than code_f32's, so that the second use
+// of a word decodes it again instead of keeping 64 decoded values in registers
+__device__ __forceinline__ float code2_f32(uint32_t word, int j) {
+    return __uint_as_float(__byte_perm(word, 0x4b800000u, 0x7640u + j)) - 16777216.0f;
+}
+
+template <int NODE, int KT>
+struct CkptSmem {
+    FcSmem<NODE, 2> node;
+    float4 b[FS_ITER][2 * KT];      // w step, w lo, step, lo of a candidate's block
+    float c[FS_ITER][2];            // sum_k w lo
+};
+
+template <int NODE, int KT>
+__global__ void __launch_bounds__(FS_WARPS * 32, 3)
+fc_soft_bwd_ckpt_kernel(const uint32_t* __restrict__ codes, uint32_t ldw, const float2* __restrict__ bounds,
+                        int64_t nblk, int64_t nv, const int32_t* __restrict__ cand, const float* __restrict__ conn,
+                        int K, int conn_ste, const float* __restrict__ params, int np_stride, int gate_hard,
+                        float inv_tau, int64_t out_dim, int64_t wire_r, const float4* __restrict__ gy,
+                        float4* __restrict__ gx, float* __restrict__ ws, int npart) {
+    constexpr int NPG = NodeSize<NODE, 2>::NPG;
+    constexpr int EK = 2 * KT;
+    __shared__ CkptSmem<NODE, KT> smem[FS_WARPS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t o = (int64_t)blockIdx.x * FS_WARPS + warp;
+    if (o >= out_dim) return;
+    const int64_t chunk = blockIdx.y;
+    const int64_t v0 = chunk * (32 * FS_ITER);
+    float* wrow = ws + (chunk * out_dim + o) * npart;
+    if (o < wire_r) {
+        if (gx)
+            for (int it = 0; it < FS_ITER; ++it) {
+                const int64_t v = v0 + it * 32 + lane;
+                if (v < nv) atomicAdd(&gx[o * nv + v], gy[o * nv + v]);
+            }
+        for (int e = lane; e < npart; e += 32) wrow[e] = 0.0f;
+        return;
+    }
+    CkptSmem<NODE, KT>& S = smem[warp];
+    stage_node<NODE, 2>(S.node, o, cand, conn, K, conn_ste, params, np_stride, gate_hard, inv_tau, lane);
+    // slot j's candidate k sits at j KT + k; unused places have weight and bounds 0 and read row 0
+    for (int e = lane; e < EK * FS_ITER; e += 32) {
+        const int it = e % FS_ITER, p = e / FS_ITER, j = p / KT, k = p % KT;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int64_t blk = chunk * FS_ITER + it;
+        if (k < K && blk < nblk) {
+            const float2 b = __ldg(&bounds[(int64_t)S.node.cand[j * K + k] * nblk + blk]);
+            const float w = S.node.w[j * K + k];
+            v = make_float4(w * b.y, w * b.x, b.y, b.x);
+        }
+        S.b[it][p] = v;
+    }
+    __syncwarp();
+    if (lane < 2 * FS_ITER) {
+        float c = 0.0f;
+        for (int k = 0; k < K; ++k) c += S.b[lane >> 1][(lane & 1) * KT + k].y;
+        S.c[lane >> 1][lane & 1] = c;
+    }
+    __syncwarp();
+    float acc_node[NPG], acc_w[EK];
+#pragma unroll
+    for (int q = 0; q < NPG; ++q) acc_node[q] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < EK; ++e) acc_w[e] = 0.0f;
+
+#pragma unroll 1
+    for (int it = 0; it < FS_ITER; ++it) {
+        const int64_t v = v0 + it * 32 + lane;
+        if (v0 + it * 32 >= nv) break;
+        __syncwarp();       // wiring and weights are read from shared memory each time, not kept
+        const bool on = v < nv;
+        uint32_t q[EK];
+#pragma unroll
+        for (int e = 0; e < EK; ++e)
+            q[e] = on && (KT == 1 || e % KT < K)
+                       ? __ldg(codes + (size_t)(uint32_t)S.node.cand[(e / KT) * K + e % KT] * ldw + v) : 0u;
+        const float4 g = on ? gy[o * nv + v] : make_float4(0.f, 0.f, 0.f, 0.f);
+        float a[4][2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float c = S.c[it][j];
+#pragma unroll
+            for (int s = 0; s < 4; ++s) a[s][j] = c;
+#pragma unroll
+            for (int k = 0; k < KT; ++k) {
+                const float wstep = S.b[it][j * KT + k].x;
+#pragma unroll
+                for (int s = 0; s < 4; ++s) a[s][j] = fmaf(wstep, code_f32(q[j * KT + k], s), a[s][j]);
+            }
+        }
+        const float gs[4] = {g.x, g.y, g.z, g.w};
+        float ga[4][2];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) node_bwd<NODE, 2>(S.node.np, a[s], gs[s], ga[s], acc_node);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float sum = (ga[0][j] + ga[1][j]) + (ga[2][j] + ga[3][j]);
+#pragma unroll
+            for (int k = 0; k < KT; ++k) {
+                if (KT > 1 && k >= K) break;
+                const int e = j * KT + k;
+                if (KT > 1) {
+                    float t = 0.0f;
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) t = fmaf(ga[s][j], code2_f32(q[e], s), t);
+                    const float4 b = S.b[it][e];
+                    acc_w[e] = fmaf(0.5f * b.z, t, fmaf(b.w, sum, acc_w[e]));
+                }
+                const float w = S.node.w[j * K + k];
+                if (gx && on && w != 0.0f)
+                    atomicAdd(&gx[(int64_t)S.node.cand[j * K + k] * nv + v],
+                              make_float4(ga[0][j] * w, ga[1][j] * w, ga[2][j] * w, ga[3][j] * w));
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
+            if (k < K) {
+                const float s = warp_sum(acc_w[j * KT + k]);
+                if (lane == 0) wrow[j * K + k] = s;
+            }
+#pragma unroll
+    for (int q = 0; q < NPG; ++q) {
+        const float s = warp_sum(acc_node[q]);
+        if (lane == 0) wrow[2 * K + q] = s;
+    }
+}
+
+template <int NODE, int KT>
+static void launch_ckpt(const FcArgs& A, const uint32_t* codes, int64_t ldw, const float2* bounds, const float* gy,
+                        float* gx, float* ws, float* gconn, float* gparams, cudaStream_t st) {
+    const int64_t nv = A.ldb / 4, nchunk = cdiv(nv, 32 * FS_ITER);
+    const int npart = 2 * A.K + NodeSize<NODE, 2>::NPG;
+    dim3 grid((unsigned)cdiv(A.out_dim, FS_WARPS), (unsigned)nchunk);
+    fc_soft_bwd_ckpt_kernel<NODE, KT><<<grid, FS_WARPS * 32, 0, st>>>(
+        codes, (uint32_t)ldw, bounds, cdiv(A.ldb, SLG_CKPT_BLOCK), nv, A.cand, A.conn, A.K, A.conn_ste, A.params,
+        np_stride_of(NODE, 2), A.gate_hard, A.inv_tau, A.out_dim, A.wire_r, reinterpret_cast<const float4*>(gy),
+        reinterpret_cast<float4*>(gx), ws, npart);
+    fc_soft_finish_kernel<NODE, 2><<<(unsigned)cdiv(A.out_dim, 128), 128, 0, st>>>(
+        ws, nchunk, A.out_dim, npart, A.K, A.conn, A.conn_ste, A.params, np_stride_of(NODE, 2), A.wire_r, gconn, gparams);
+}
+
+}  // namespace slg
+
+using namespace slg;
+
+extern "C" int32_t slg_fc_soft_bwd_ckpt_built(int32_t K, int32_t node, int32_t arity) {
+    return arity == 2 && K >= 1 && K <= 8 && (node == N_GATE16 || node == N_WALSH || node == N_MULTI || node == N_HYBRID);
+}
+
+extern "C" int slg_fc_soft_bwd_ckpt(const uint8_t* codes, int64_t ldc, const float* bounds, int64_t in_dim, int64_t ldb,
+                                    const int32_t* cand, const float* conn, int32_t K, int32_t conn_ste, int32_t node,
+                                    int32_t arity, const float* params, int32_t gate_hard, float inv_tau,
+                                    int64_t out_dim, int64_t wire_r, const float* gy, float* gx, float* gconn,
+                                    float* gparams, void* workspace, int64_t workspace_bytes, void* stream) {
+    const char* name = "slg_fc_soft_bwd_ckpt";
+    if (in_dim <= 0 || out_dim < 0 || ldb <= 0 || K <= 0 || wire_r < 0) return set_error(SLG_ERR_ARG, "%s: bad sizes", name);
+    if (!slg_fc_soft_bwd_ckpt_built(K, node, arity))
+        return set_error(SLG_ERR_UNSUPPORTED, "%s: node %d arity %d K=%d not built", name, node, arity, K);
+    if (ldb % 4 || ldc % 4) return set_error(SLG_ERR_ALIGN, "%s: ldb and ldc must be multiples of 4", name);
+    if (ldc < ldb) return set_error(SLG_ERR_ARG, "%s: ldc < ldb", name);
+    if (ldc / 4 >= (1ll << 32)) return set_error(SLG_ERR_ARG, "%s: rows too long", name);
+    if (conn_ste < 0 || conn_ste > 2) return set_error(SLG_ERR_ARG, "%s: conn_ste %d not in 0..2", name, conn_ste);
+    if (wire_r > 0 && (wire_r > in_dim || wire_r > out_dim)) return set_error(SLG_ERR_ARG, "%s: wire_r exceeds a width", name);
+    if (cdiv(ldb / 4, 32 * FS_ITER) > 65535) return set_error(SLG_ERR_ARG, "%s: batch too large", name);
+    if (!codes || !bounds || !cand || !params || !gy || !gparams || !workspace)
+        return set_error(SLG_ERR_ARG, "%s: null pointer", name);
+    if (conn && !gconn) return set_error(SLG_ERR_ARG, "%s: gconn required with conn", name);
+    if (!aligned16(gy) || (gx && !aligned16(gx)) || (reinterpret_cast<uintptr_t>(codes) & 3u) ||
+        (reinterpret_cast<uintptr_t>(bounds) & 7u))
+        return set_error(SLG_ERR_ALIGN, "%s: gy/gx/codes/bounds misaligned", name);
+    const int64_t need = slg_fc_soft_workspace_bytes(ldb, K, node, arity, out_dim);
+    if (workspace_bytes < need)
+        return set_error(SLG_ERR_WORKSPACE, "%s: workspace %lld < %lld bytes", name, (long long)workspace_bytes,
+                         (long long)need);
+    if (out_dim == 0) return SLG_OK;
+    const FcArgs A{nullptr, in_dim, ldb, cand, conn, K, conn_ste, params, gate_hard, inv_tau, out_dim, wire_r};
+    const uint32_t* c = reinterpret_cast<const uint32_t*>(codes);
+    const float2* b = reinterpret_cast<const float2*>(bounds);
+    float* ws = static_cast<float*>(workspace);
+    cudaStream_t s = as_stream(stream);
+    auto go = [&](auto node_tag) {
+        constexpr int NODE = decltype(node_tag)::value;
+        if (K == 1) launch_ckpt<NODE, 1>(A, c, ldc / 4, b, gy, gx, ws, gconn, gparams, s);
+        else if (K <= 4) launch_ckpt<NODE, 4>(A, c, ldc / 4, b, gy, gx, ws, gconn, gparams, s);
+        else launch_ckpt<NODE, 8>(A, c, ldc / 4, b, gy, gx, ws, gconn, gparams, s);
+    };
+    switch (node) {
+        case N_GATE16: go(std::integral_constant<int, N_GATE16>()); break;
+        case N_WALSH: go(std::integral_constant<int, N_WALSH>()); break;
+        case N_MULTI: go(std::integral_constant<int, N_MULTI>()); break;
+        default: go(std::integral_constant<int, N_HYBRID>()); break;
+    }
+    return check_launch(name);
+}

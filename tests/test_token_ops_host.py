@@ -85,15 +85,12 @@ def test_c_entry_points_refuse_bad_arguments(L):
         _p(codes), ldc, _p(bounds), rows, cols, _p(x), dt, ldx, _p(0))
     assert load(cols=-1) == 1 and load(ldc=11) == 2 and load(dt=-1) == 3 and load(x=0) == 1
     # beams
-    need = L.slg_beam_step_workspace_bytes(2, 4, 50, 4)
-    step = lambda B=2, k=4, V=50, ldx=50, w=4, dt=0, fin=0, eos=-1, x=256, size=need: L.slg_beam_step(     # noqa: E731
-        _p(x), dt, B, k, V, ldx, _p(256), _p(fin), eos, w, _p(256), _p(256), _p(256), _p(0), _p(256), size, _p(0))
-    assert step(B=-1) == 1 and step(V=0) == 1 and step(ldx=49) == 1 and step(k=33, size=1 << 20) == 3
-    assert step(w=33, size=1 << 20) == 3 and step(k=1, V=2, ldx=2, w=3) == 1 and step(dt=5) == 3
+    step = lambda B=2, k=4, V=50, ldx=50, w=4, dt=0, fin=0, eos=-1, x=256: L.slg_beam_step(                # noqa: E731
+        _p(x), dt, B, k, V, ldx, _p(256), _p(fin), eos, w, _p(256), _p(256), _p(256), _p(0), _p(0))
+    assert step(B=-1) == 1 and step(V=0) == 1 and step(ldx=49) == 1 and step(k=33) == 3 and step(w=33) == 3
+    assert step(k=1, V=2, ldx=2, w=3) == 1 and step(dt=5) == 3 and step(V=1 << 27, ldx=1 << 27) == 3
     assert step(fin=256, eos=-1) == 1 and step(fin=256, eos=50) == 1 and step(x=0) == 1
     assert step(B=0, x=0) == 0
-    if need:
-        assert step(size=need - 1) == 5
     rows = lambda i=256, o=512, nb=16, B=2: L.slg_beam_reorder_rows(_p(i), nb, _p(256), B, 4, 4, _p(o), _p(0))   # noqa: E731
     assert rows(i=0) == 1 and rows(o=256) == 1 and rows(nb=-1) == 1 and rows(B=0) == 0 and rows(nb=0) == 0
     assert L.slg_beam_reorder_features(_p(256), 3, 7, _p(256), 2, 4, 4, _p(512), 8, _p(0)) == 1       # rows too short
