@@ -156,29 +156,31 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
                 const float ref = m > -CUDART_INF_F ? m : 0.0f;
 #pragma unroll
                 for (int i = 0; i < BM_PER; ++i) s += __expf(x[i] - ref);
-                // search: the lane's best untaken logit, its lowest index first
-                uint32_t left = valid;
-                uint64_t k = 0;
-                auto next = [&]() {
-                    float v = -CUDART_INF_F;
-                    int at = -1;
-#pragma unroll
-                    for (int i = 0; i < BM_PER; ++i)
-                        if ((left >> i & 1u) && (at < 0 || x[i] > v)) { v = x[i]; at = i; }
-                    k = at < 0 ? 0 : cand_key(v, (uint32_t)(base + (at / E) * 32 * E + at % E));
-                    if (at >= 0) left &= ~(1u << at);
-                };
+                // Logits that can enter the list beat its last entry; while it is being filled,
+                // also the `width`-th largest of the lanes' maxima (so many logits reach that).
                 uint64_t bar = __shfl_sync(0xffffffffu, list, width - 1);
                 if (!__any_sync(0xffffffffu, valid && ordered(top) >= (uint32_t)(bar >> 32))) continue;
-                next();
-                for (;;) {
-                    const uint64_t w = warp_max(k);
-                    if (w <= bar) break;                            // also when nothing is left (0)
-                    if (k == w) next();
-                    const int at = __popc(__ballot_sync(0xffffffffu, lane < width && list > w));
-                    const uint64_t up = __shfl_up_sync(0xffffffffu, list, 1);
-                    if (lane < width && lane >= at) list = lane == at ? w : up;
-                    bar = __shfl_sync(0xffffffffu, list, width - 1);
+                uint32_t reach = (uint32_t)(bar >> 32);
+                if (bar == 0) {
+                    uint32_t t = valid ? ordered(top) : 0u;
+                    for (int n = 0; n < width; ++n) {
+                        reach = __reduce_max_sync(0xffffffffu, t);
+                        if (lane == __ffs(__ballot_sync(0xffffffffu, t == reach)) - 1) t = 0;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < BM_PER; ++i) {
+                    uint32_t in = __ballot_sync(0xffffffffu, (valid >> i & 1u) && ordered(x[i]) >= reach);
+                    if (in == 0) continue;
+                    const uint64_t k = cand_key(x[i], (uint32_t)(base + (i / E) * 32 * E + i % E));
+                    for (; in; in &= in - 1) {
+                        const uint64_t w = __shfl_sync(0xffffffffu, k, __ffs(in) - 1);
+                        if (w <= bar) continue;
+                        const int at = __popc(__ballot_sync(0xffffffffu, lane < width && list > w));
+                        const uint64_t up = __shfl_up_sync(0xffffffffu, list, 1);
+                        if (lane < width && lane >= at) list = lane == at ? w : up;
+                        bar = __shfl_sync(0xffffffffu, list, width - 1);
+                    }
                 }
             }
         }
@@ -288,36 +290,44 @@ __global__ void reorder_rows_kernel(const W* __restrict__ in, int64_t words, con
         out[r * words + c] = src[c];
 }
 
-// Column r of every feature row = column (r / width) * beams + parents[r]; padding columns 0.
-__global__ void reorder_features_kernel(const float* __restrict__ in, int64_t F, int64_t ldi, int64_t n,
-                                        const int64_t* __restrict__ parents, int beams, int width,
-                                        float* __restrict__ out, int64_t ldo) {
-    const int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (r >= ldo) return;
-    int64_t src = -1;
-    if (r < n) {
-        const int64_t p = parents[r];
-        src = (r / width) * beams + (p >= 0 && p < beams ? p : 0);
-    }
-    for (int64_t f = blockIdx.y; f < F; f += gridDim.y) out[f * ldo + r] = src >= 0 ? in[f * ldi + src] : 0.0f;
+// The sample that sample r of the output is
+__device__ __forceinline__ int64_t beam_source(const int64_t* __restrict__ parents, uint32_t r, int beams, int width) {
+    const int64_t p = parents[r];
+    return (int64_t)(r / (uint32_t)width) * beams + (p >= 0 && p < beams ? p : 0);
 }
 
-// The same on bits: bit r of every packed row; a warp builds 32 samples of a row by ballot.
-__global__ void reorder_packed_kernel(const uint32_t* __restrict__ in, int64_t F, int64_t ldi, int64_t n,
-                                      const int64_t* __restrict__ parents, int beams, int width,
-                                      uint32_t* __restrict__ out, int64_t ldo) {
+// Column r of every feature row = column source(r); padding columns 0.  A thread keeps its
+// column and walks rows, so the source is worked out once.
+constexpr int RF_ROWS = 8;              // rows of a CTA per step
+__global__ void __launch_bounds__(32 * RF_ROWS)
+reorder_features_kernel(const float* __restrict__ in, int64_t F, int64_t ldi, int64_t n,
+                        const int64_t* __restrict__ parents, int beams, int width, float* __restrict__ out,
+                        int64_t ldo) {
+    const int64_t r = (int64_t)blockIdx.x * 32 + threadIdx.x;
+    if (r >= ldo) return;
+    const bool on = r < n;
+    const int64_t src = on ? beam_source(parents, (uint32_t)r, beams, width) : 0;
+#pragma unroll 4
+    for (int64_t f = (int64_t)blockIdx.y * RF_ROWS + threadIdx.y; f < F; f += (int64_t)gridDim.y * RF_ROWS)
+        out[f * ldo + r] = on ? __ldg(&in[f * ldi + src]) : 0.0f;
+}
+
+// The same on bits: a warp builds one 32-sample word of a row by ballot, for many rows.
+constexpr int RP_WARPS = 8;
+__global__ void __launch_bounds__(RP_WARPS * 32)
+reorder_packed_kernel(const uint32_t* __restrict__ in, int64_t F, int64_t ldi, int64_t n,
+                      const int64_t* __restrict__ parents, int beams, int width, uint32_t* __restrict__ out,
+                      int64_t ldo) {
     const int lane = threadIdx.x & 31;
     const int64_t w = blockIdx.x;                           // 32-bit word of the output rows
     const int64_t r = w * 32 + lane;
-    int64_t src = -1;
-    if (r < n) {
-        const int64_t p = parents[r];
-        src = (r / width) * beams + (p >= 0 && p < beams ? p : 0);
-    }
-    const int warps = blockDim.x >> 5;
-    for (int64_t f = (int64_t)blockIdx.y * warps + (threadIdx.x >> 5); f < F; f += (int64_t)gridDim.y * warps) {
-        const bool bit = src >= 0 && ((in[f * ldi + (src >> 5)] >> (src & 31)) & 1u);
-        const uint32_t word = __ballot_sync(0xffffffffu, bit);
+    const bool on = r < n;
+    const int64_t src = on ? beam_source(parents, (uint32_t)r, beams, width) : 0;
+    const uint32_t bit = (uint32_t)src & 31u;
+    in += src >> 5;
+#pragma unroll 8
+    for (int64_t f = (int64_t)blockIdx.y * RP_WARPS + (threadIdx.x >> 5); f < F; f += (int64_t)gridDim.y * RP_WARPS) {
+        const uint32_t word = __ballot_sync(0xffffffffu, on && (__ldg(&in[f * ldi]) >> bit & 1u));
         if (lane == 0) out[f * ldo + w] = word;
     }
 }
@@ -390,8 +400,8 @@ extern "C" int slg_beam_reorder_features(const float* in, int64_t F, int64_t ldi
     if (st) return st;
     if (F < 0 || ldi < B * beams || ldo < B * width)
         return set_error(SLG_ERR_ARG, "slg_beam_reorder_features: bad sizes");
-    const dim3 grid((unsigned)cdiv(ldo, 128), (unsigned)std::min<int64_t>(F, 8192));
-    reorder_features_kernel<<<grid, 128, 0, as_stream(stream)>>>(in, F, ldi, B * width, parents, beams, width, out, ldo);
+    const dim3 grid((unsigned)cdiv(ldo, 32), (unsigned)std::min<int64_t>(cdiv(F, RF_ROWS * 4), 65535));
+    reorder_features_kernel<<<grid, dim3(32, RF_ROWS), 0, as_stream(stream)>>>(in, F, ldi, B * width, parents, beams, width, out, ldo);
     return check_launch("slg_beam_reorder_features");
 }
 
@@ -402,8 +412,8 @@ extern "C" int slg_beam_reorder_packed(const uint64_t* in, int64_t F, int64_t ld
     if (st) return st;
     if (F < 0 || ldi * 64 < B * beams || ldo * 64 < B * width)
         return set_error(SLG_ERR_ARG, "slg_beam_reorder_packed: bad sizes");
-    const dim3 grid((unsigned)(2 * ldo), (unsigned)std::min<int64_t>(cdiv(F, 8), 4096));
-    reorder_packed_kernel<<<grid, 256, 0, as_stream(stream)>>>(reinterpret_cast<const uint32_t*>(in), F, 2 * ldi,
+    const dim3 grid((unsigned)(2 * ldo), (unsigned)std::min<int64_t>(cdiv(F, RP_WARPS * 8), 65535));
+    reorder_packed_kernel<<<grid, RP_WARPS * 32, 0, as_stream(stream)>>>(reinterpret_cast<const uint32_t*>(in), F, 2 * ldi,
                                                                B * width, parents, beams, width,
                                                                reinterpret_cast<uint32_t*>(out), 2 * ldo);
     return check_launch("slg_beam_reorder_packed");

@@ -15,7 +15,7 @@ constexpr int CK_BLOCK = SLG_CKPT_BLOCK;        // columns per (lo, step)
 constexpr int CK_WARPS = 8;
 constexpr float CK_TINY = 7.888609052210118e-31f;    // 2^-100
 
-static_assert(CK_BLOCK == 128, "a warp handles a block, 4 values per lane");
+static_assert(CK_BLOCK == 128, "a warp covers a block, 4 values per lane");
 
 template <typename T>
 __device__ __forceinline__ void load4(const T* __restrict__ p, int64_t c, int64_t cols, bool vec, float (&v)[4]) {
@@ -34,47 +34,83 @@ __device__ __forceinline__ void load4(const T* __restrict__ p, int64_t c, int64_
     }
 }
 
-// one warp = one block of one row
+__device__ __forceinline__ float warp_min_f32(float v) {
+    float r;
+    asm("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float warp_max_nan_f32(float v) {        // NaN when any lane has one
+    float r;
+    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float max_nan_f32(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// A warp handles CK_UNIT consecutive blocks (all loads first): with one block per warp the
+// kernels ran at 41% and 72% of the copy rate on 10,000 x 65,536 fp32.
+constexpr int CK_UNIT = 4;
+
+// row and block of block number q (32-bit division where it suffices)
+__device__ __forceinline__ void block_of(int64_t q, int64_t nblk, int64_t& row, int64_t& blk) {
+    row = q < (1ll << 32) && nblk < (1ll << 32) ? (int64_t)((uint32_t)q / (uint32_t)nblk) : q / nblk;
+    blk = q - row * nblk;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(CK_WARPS * 32)
 ckpt_store_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t ldx, int vec,
                   uint32_t* __restrict__ codes, int64_t ldw, float2* __restrict__ bounds, int64_t nblk) {
     const int lane = threadIdx.x & 31;
-    const int64_t q = (int64_t)blockIdx.x * CK_WARPS + (threadIdx.x >> 5);
-    if (q >= rows * nblk) return;
-    const int64_t row = q / nblk, blk = q - row * nblk;
-    const int64_t c = blk * CK_BLOCK + lane * 4;
-    float v[4];
-    load4(x + row * ldx, c, cols, vec, v);
-    float lo = CUDART_INF_F, hi = -CUDART_INF_F;
-    bool bad = false;
+    const int64_t q0 = ((int64_t)blockIdx.x * CK_WARPS + (threadIdx.x >> 5)) * CK_UNIT;
+    const int64_t total = rows * nblk;
+    if (q0 >= total) return;
+    int64_t row, blk;
+    block_of(q0, nblk, row, blk);
+    float v[CK_UNIT][4];
+    int64_t word_at[CK_UNIT];       // the lane's code word, -1: none
+    int n[CK_UNIT];                 // its values
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (c + j < cols) {
-            lo = fminf(lo, v[j]);
-            hi = fmaxf(hi, v[j]);
-            bad |= !isfinite(v[j]);
-        }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    for (int u = 0; u < CK_UNIT; ++u) {
+        const int64_t c = blk * CK_BLOCK + lane * 4;
+        const bool on = q0 + u < total && c < cols;
+        n[u] = on ? (int)(cols - c < 4 ? cols - c : 4) : 0;
+        word_at[u] = row * ldw + (c >> 2);
+        if (on) load4(x + row * ldx, c, cols, vec, v[u]);
+        if (++blk == nblk) { blk = 0; ++row; }
     }
-    const float range = __fsub_rn(hi, lo);
-    bad = __any_sync(0xffffffffu, bad) || !isfinite(range);
-    float step = __fmul_rn(range, 1.0f / 255.0f);
-    const bool flat = bad || step < CK_TINY;
-    const float inv = flat ? 0.0f : __fdiv_rn(255.0f, range);
-    uint32_t word = 0;
+    float2 mine = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (!flat && c + j < cols) {
-            const float code = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(v[j], lo), inv)), 0.0f), 255.0f);
-            word |= (uint32_t)code << (8 * j);
-        }
-    if (c < cols) codes[row * ldw + (c >> 2)] = word;
-    if (lane == 0)
-        bounds[q] = bad ? make_float2(CUDART_NAN_F, CUDART_NAN_F) : make_float2(lo, flat ? 0.0f : step);
+    for (int u = 0; u < CK_UNIT; ++u) {
+        float lo = CUDART_INF_F, hi = -CUDART_INF_F;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < n[u]) {
+                lo = fminf(lo, v[u][j]);
+                hi = max_nan_f32(hi, v[u][j]);
+            }
+        lo = warp_min_f32(lo);
+        hi = warp_max_nan_f32(hi);
+        const float range = __fsub_rn(hi, lo);              // NaN or infinite: something is not finite
+        const bool bad = !isfinite(range);
+        const float step = __fmul_rn(range, 1.0f / 255.0f);
+        const bool flat = bad || step < CK_TINY;
+        const float inv = flat ? 0.0f : __fdiv_rn(255.0f, range);
+        uint32_t word = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (!flat && j < n[u]) {
+                const float code = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(v[u][j], lo), inv)), 0.0f), 255.0f);
+                word |= (uint32_t)code << (8 * j);
+            }
+        if (n[u]) codes[word_at[u]] = word;
+        if (lane == u)
+            mine = bad ? make_float2(CUDART_NAN_F, CUDART_NAN_F) : make_float2(lo, flat ? 0.0f : step);
+    }
+    if (lane < CK_UNIT && q0 + lane < total) bounds[q0 + lane] = mine;
 }
 
 template <typename T>
@@ -82,24 +118,39 @@ __global__ void __launch_bounds__(CK_WARPS * 32)
 ckpt_load_kernel(const uint32_t* __restrict__ codes, int64_t ldw, const float2* __restrict__ bounds, int64_t rows,
                  int64_t cols, int64_t nblk, T* __restrict__ x, int64_t ldx, int vec) {
     const int lane = threadIdx.x & 31;
-    const int64_t q = (int64_t)blockIdx.x * CK_WARPS + (threadIdx.x >> 5);
-    if (q >= rows * nblk) return;
-    const int64_t row = q / nblk, blk = q - row * nblk;
-    const int64_t c = blk * CK_BLOCK + lane * 4;
-    if (c >= cols) return;
-    const uint32_t word = __ldg(&codes[row * ldw + (c >> 2)]);
-    const float2 b = __ldg(&bounds[q]);
-    float v[4];
+    const int64_t q0 = ((int64_t)blockIdx.x * CK_WARPS + (threadIdx.x >> 5)) * CK_UNIT;
+    const int64_t total = rows * nblk;
+    if (q0 >= total) return;
+    int64_t row, blk;
+    block_of(q0, nblk, row, blk);
+    uint32_t word[CK_UNIT];
+    float2 b[CK_UNIT];
+    T* p[CK_UNIT];
+    int n[CK_UNIT];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = __fadd_rn(__fmul_rn((float)((word >> (8 * j)) & 255u), b.y), b.x);
-    T* p = x + row * ldx + c;
-    if (vec && c + 4 <= cols) {
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-        else *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(v), pack2<T>(v + 2));
-    } else {
+    for (int u = 0; u < CK_UNIT; ++u) {
+        const int64_t c = blk * CK_BLOCK + lane * 4;
+        const bool on = q0 + u < total && c < cols;
+        n[u] = on ? (int)(cols - c < 4 ? cols - c : 4) : 0;
+        p[u] = x + row * ldx + c;
+        word[u] = on ? __ldg(&codes[row * ldw + (c >> 2)]) : 0u;
+        b[u] = on ? __ldg(&bounds[q0 + u]) : make_float2(0.f, 0.f);
+        if (++blk == nblk) { blk = 0; ++row; }
+    }
+#pragma unroll
+    for (int u = 0; u < CK_UNIT; ++u) {
+        float v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (c + j < cols) p[j] = from_f32<T>(v[j]);
+            v[j] = __fadd_rn(__fmul_rn((float)((word[u] >> (8 * j)) & 255u), b[u].y), b[u].x);
+        if (vec && n[u] == 4) {
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p[u]) = make_float4(v[0], v[1], v[2], v[3]);
+            else *reinterpret_cast<uint2*>(p[u]) = make_uint2(pack2<T>(v), pack2<T>(v + 2));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < n[u]) p[u][j] = from_f32<T>(v[j]);
+        }
     }
 }
 
@@ -134,7 +185,7 @@ extern "C" int slg_ckpt_store(const void* x, int32_t dtype, int64_t rows, int64_
     for_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         const int vec = ldx % 4 == 0 && aligned_to(x, 4 * sizeof(T));
-        ckpt_store_kernel<T><<<(unsigned)cdiv(rows * nblk, CK_WARPS), CK_WARPS * 32, 0, s>>>(
+        ckpt_store_kernel<T><<<(unsigned)cdiv(rows * nblk, CK_WARPS * CK_UNIT), CK_WARPS * 32, 0, s>>>(
             (const T*)x, rows, cols, ldx, vec, reinterpret_cast<uint32_t*>(codes), ldc / 4,
             reinterpret_cast<float2*>(bounds), nblk);
     });
@@ -152,7 +203,7 @@ extern "C" int slg_ckpt_load(const uint8_t* codes, int64_t ldc, const float* bou
     for_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         const int vec = ldx % 4 == 0 && aligned_to(x, 4 * sizeof(T));
-        ckpt_load_kernel<T><<<(unsigned)cdiv(rows * nblk, CK_WARPS), CK_WARPS * 32, 0, s>>>(
+        ckpt_load_kernel<T><<<(unsigned)cdiv(rows * nblk, CK_WARPS * CK_UNIT), CK_WARPS * 32, 0, s>>>(
             reinterpret_cast<const uint32_t*>(codes), ldc / 4, reinterpret_cast<const float2*>(bounds), rows, cols,
             nblk, (T*)x, ldx, vec);
     });

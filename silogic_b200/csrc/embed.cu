@@ -14,57 +14,70 @@ constexpr int EM_THREADS = 256;
 constexpr int EM_UNROLL = 4;        // 16-byte vectors per thread of the lookup
 
 // ------------------------------------------------------------------ lookup
-// One thread = EM_UNROLL 16-byte vectors of the output; VEC: rows are whole vectors.
-template <typename T, typename I, bool VEC>
+// One thread = EM_UNROLL 16-byte vectors of the output.  VEC: rows are whole vectors (`per` of
+// them); otherwise a vector may cross rows and its values are read one by one.  Below 2^32
+// vectors (S = uint32_t) the row of a vector is one 32-bit division; the 64-bit one alone
+// takes longer than the copy.
+template <typename T, typename I, typename S, bool VEC>
 __global__ void __launch_bounds__(EM_THREADS)
 embed_fwd_kernel(const I* __restrict__ ids, int64_t N, const T* __restrict__ w, int64_t V, int64_t D,
-                 float scale, T* __restrict__ y) {
+                 S per, float scale, T* __restrict__ y) {
     constexpr int E = Pack16<T>::E;
-    const int64_t total = N * D;
-    const int64_t base = ((int64_t)blockIdx.x * EM_THREADS * EM_UNROLL + threadIdx.x) * E;
+    const S first = (S)blockIdx.x * (EM_THREADS * EM_UNROLL) + threadIdx.x;
+    if constexpr (VEC) {
+        const S total = (S)N * per;
+        uint4 u[EM_UNROLL];
+        bool ok[EM_UNROLL];
 #pragma unroll
-    for (int u = 0; u < EM_UNROLL; ++u) {
-        const int64_t e0 = base + (int64_t)u * EM_THREADS * E;
-        if (e0 >= total) continue;
-        int64_t i = e0 / D, c = e0 - i * D;
-        int64_t t = (int64_t)ids[i];
-        float v[E];
-        if constexpr (VEC) {
-            if (t >= 0 && t < V) unpack16<T>(__ldg(reinterpret_cast<const uint4*>(w + t * D + c)), v);
-            else
-#pragma unroll
-                for (int j = 0; j < E; ++j) v[j] = CUDART_NAN_F;
-        } else {
-#pragma unroll
-            for (int j = 0; j < E; ++j) {
-                v[j] = e0 + j >= total ? 0.0f : t >= 0 && t < V ? to_f32(w[t * D + c]) : CUDART_NAN_F;
-                if (++c == D && e0 + j + 1 < total) { c = 0; t = (int64_t)ids[++i]; }
+        for (int q = 0; q < EM_UNROLL; ++q) {
+            const S k = first + q * EM_THREADS;
+            ok[q] = false;
+            u[q] = make_uint4(0, 0, 0, 0);
+            if (k < total) {
+                const S i = k / per, c = k - i * per;
+                const int64_t t = (int64_t)ids[i];
+                ok[q] = t >= 0 && t < V;
+                if (ok[q]) u[q] = __ldg(reinterpret_cast<const uint4*>(w + t * D) + c);
             }
         }
 #pragma unroll
-        for (int j = 0; j < E; ++j) v[j] *= scale;
-        if (e0 + E <= total) *reinterpret_cast<uint4*>(y + e0) = pack16<T>(v);
-        else
+        for (int q = 0; q < EM_UNROLL; ++q) {
+            const S k = first + q * EM_THREADS;
+            if (k >= total) continue;
+            float v[E];
+            unpack16<T>(u[q], v);
 #pragma unroll
-            for (int j = 0; j < E; ++j)
-                if (e0 + j < total) y[e0 + j] = from_f32<T>(v[j]);
+            for (int j = 0; j < E; ++j) v[j] = ok[q] ? v[j] * scale : CUDART_NAN_F;
+            __stcs(reinterpret_cast<uint4*>(y) + k, pack16<T>(v));
+        }
+    } else {
+        const int64_t total = N * D;
+#pragma unroll
+        for (int q = 0; q < EM_UNROLL; ++q) {
+            const int64_t e0 = (int64_t)(first + q * EM_THREADS) * E;
+            if (e0 >= total) continue;
+            int64_t i = total < (1ll << 32) ? (int64_t)((uint32_t)e0 / (uint32_t)D) : e0 / D, c = e0 - i * D;
+            int64_t t = (int64_t)ids[i];
+            float v[E];
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                v[j] = e0 + j >= total ? 0.0f : t >= 0 && t < V ? to_f32(w[t * D + c]) * scale : CUDART_NAN_F;
+                if (++c == D && e0 + j + 1 < total) { c = 0; t = (int64_t)ids[++i]; }
+            }
+            if (e0 + E <= total) *reinterpret_cast<uint4*>(y + e0) = pack16<T>(v);
+            else
+#pragma unroll
+                for (int j = 0; j < E; ++j)
+                    if (e0 + j < total) y[e0 + j] = from_f32<T>(v[j]);
+        }
     }
 }
 
 // -------------------------------------------------------------------- sort
-// Stable LSD radix sort of (token, position), 8 bits a pass.  Tokens that get no gradient
-// (padding, out of range) carry the key V and sort past every row.
-constexpr int RS_THREADS = 256;
-constexpr int RS_WARPS = RS_THREADS / 32;
-constexpr int RS_PER = 16;                          // keys per thread of a tile
-constexpr int RS_TILE = RS_THREADS * RS_PER;
-constexpr int RS_BINS = 256;
-constexpr int RS_MAX_TILES = 256;
-
-__host__ __device__ inline int64_t rs_span(int64_t N) {   // keys per CTA: whole tiles, at most RS_MAX_TILES CTAs
-    return RS_TILE * cdiv(cdiv(N, RS_TILE), RS_MAX_TILES);
-}
-
+// Tokens that get no gradient (padding, out of range) carry the key V and sort past every
+// row.  Up to RK_MAX tokens every token counts the tokens before it in sorted order (N^2
+// comparisons, one launch); above, a stable LSD radix sort of (token, position) with digits
+// of at most 9 bits, so two passes (four launches) sort vocabularies below 2^18.
 template <typename I>
 struct KeysOfIds {
     const I* ids; int64_t V; int64_t pad;
@@ -80,32 +93,102 @@ struct KeysOfPairs {
     __device__ __forceinline__ uint32_t pos(int64_t i) const { return p[i]; }
 };
 
+constexpr int RK_MAX = 8192;
+constexpr int RK_THREADS = 256;
+constexpr int RK_WARPS = RK_THREADS / 32;
+
+// A CTA ranks 32 tokens (one per lane), each warp against its eighth of the batch: tokens
+// at earlier positions count when they are <= its own, later ones when they are <.
+template <typename I>
+__global__ void __launch_bounds__(RK_THREADS)
+rank_sort_kernel(KeysOfIds<I> src, int N, uint32_t* __restrict__ ko, uint32_t* __restrict__ po) {
+    __shared__ alignas(16) uint32_t key[RK_MAX];
+    __shared__ int part[RK_WARPS][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n4 = (N + 3) & ~3;
+    for (int i = threadIdx.x; i < n4; i += RK_THREADS) key[i] = i < N ? src.key(i) : 0xffffffffu;
+    __syncthreads();
+    const int i0 = blockIdx.x * 32, i = i0 + lane;
+    const uint32_t mine = i < N ? key[i] : 0u;
+    const int a = n4 / 4 * warp / RK_WARPS, b = n4 / 4 * (warp + 1) / RK_WARPS;    // groups of 4 keys
+    const uint4* k4 = reinterpret_cast<const uint4*>(key);
+    int rank = 0;
+    const int lo = min(max(i0 / 4, a), b), hi = min(max(i0 / 4 + 8, a), b);        // the CTA's own tokens
+#pragma unroll 4
+    for (int g = a; g < lo; ++g) {
+        const uint4 k = k4[g];
+        rank += (k.x <= mine) + (k.y <= mine) + (k.z <= mine) + (k.w <= mine);
+    }
+    for (int g = lo; g < hi; ++g)
+        for (int j = 4 * g; j < 4 * g + 4; ++j) rank += key[j] < mine || (key[j] == mine && j < i);
+#pragma unroll 4
+    for (int g = hi; g < b; ++g) {
+        const uint4 k = k4[g];
+        rank += (k.x < mine) + (k.y < mine) + (k.z < mine) + (k.w < mine);
+    }
+    part[warp][lane] = rank;
+    __syncthreads();
+    if (warp == 0 && i < N) {
+        int at = 0;
+#pragma unroll
+        for (int w = 0; w < RK_WARPS; ++w) at += part[w][lane];
+        ko[at] = mine;
+        po[at] = (uint32_t)i;
+    }
+}
+
+constexpr int RS_THREADS = 512;
+constexpr int RS_WARPS = RS_THREADS / 32;
+constexpr int RS_PER = 4;                           // keys per thread of a tile
+constexpr int RS_TILE = RS_THREADS * RS_PER;
+constexpr int RS_BITS = 9;
+constexpr int RS_BINS = 1 << RS_BITS;               // one per thread
+constexpr int RS_MAX_TILES = 128;
+
+__host__ __device__ inline int64_t rs_span(int64_t N) {   // keys per CTA: whole tiles, at most RS_MAX_TILES CTAs
+    return RS_TILE * cdiv(cdiv(N, RS_TILE), RS_MAX_TILES);
+}
+
 // hist[cta][digit]
 template <typename S>
 __global__ void __launch_bounds__(RS_THREADS)
-radix_count_kernel(S src, int64_t N, int64_t span, int shift, uint32_t* __restrict__ hist) {
+radix_count_kernel(S src, int64_t N, int64_t span, int shift, uint32_t mask, uint32_t* __restrict__ hist) {
     __shared__ uint32_t h[RS_BINS];
     h[threadIdx.x] = 0;
     __syncthreads();
     const int64_t a = (int64_t)blockIdx.x * span, b = a + span < N ? a + span : N;
-    for (int64_t i = a + threadIdx.x; i < b; i += RS_THREADS) atomicAdd(&h[(src.key(i) >> shift) & 255u], 1u);
+#pragma unroll 4
+    for (int64_t i = a + threadIdx.x; i < b; i += RS_THREADS) atomicAdd(&h[(src.key(i) >> shift) & mask], 1u);
     __syncthreads();
     hist[(int64_t)blockIdx.x * RS_BINS + threadIdx.x] = h[threadIdx.x];
 }
 
 // Thread d owns digit d.  Its first slot is the number of keys with a smaller digit plus
 // those with digit d in earlier CTAs; inside a tile a warp owns consecutive keys, ranks
-// them 32 at a time by matching digits, and warps follow one another: the order is stable.
+// them 32 at a time among the lanes with the same digit (one ballot per bit: match_any is
+// several times slower on 32 different digits), and warps follow one another: the order is stable.
 template <typename S>
 __global__ void __launch_bounds__(RS_THREADS)
-radix_scatter_kernel(S src, int64_t N, int64_t span, int shift, const uint32_t* __restrict__ hist,
+radix_scatter_kernel(S src, int64_t N, int64_t span, int shift, int bits, const uint32_t* __restrict__ hist,
                      uint32_t* __restrict__ ko, uint32_t* __restrict__ po) {
     __shared__ uint32_t base[RS_BINS];
     __shared__ uint32_t cnt[RS_WARPS][RS_BINS];
     __shared__ uint32_t wsum[RS_WARPS];
     const int d = threadIdx.x, warp = d >> 5, lane = d & 31;
+    const uint32_t mask = (1u << bits) - 1u;
+    const int64_t a = (int64_t)blockIdx.x * span, b = a + span < N ? a + span : N;
+    uint32_t key[RS_PER], pos[RS_PER];
+    auto load = [&](int64_t w0) {
+#pragma unroll
+        for (int j = 0; j < RS_PER; ++j) {
+            const bool on = w0 + 32 * j < b;
+            key[j] = on ? src.key(w0 + 32 * j) : 0u;
+            pos[j] = on ? src.pos(w0 + 32 * j) : 0u;
+        }
+    };
+    load(a + warp * (32 * RS_PER) + lane);
     uint32_t before = 0, all = 0;
-#pragma unroll 8
+#pragma unroll 16
     for (int t = 0; t < (int)gridDim.x; ++t) {
         const uint32_t c = hist[(int64_t)t * RS_BINS + d];
         before += t < (int)blockIdx.x ? c : 0u;
@@ -122,24 +205,30 @@ radix_scatter_kernel(S src, int64_t N, int64_t span, int shift, const uint32_t* 
     for (int q = 0; q < warp; ++q) inc += wsum[q];
     base[d] = inc - all + before;
 
-    const int64_t a = (int64_t)blockIdx.x * span, b = a + span < N ? a + span : N;
     for (int64_t t0 = a; t0 < b; t0 += RS_TILE) {
+        const int64_t w0 = t0 + warp * (32 * RS_PER) + lane;
+        if (t0 > a) load(w0);
 #pragma unroll
         for (int q = 0; q < RS_WARPS; ++q) cnt[q][d] = 0;
         __syncthreads();
-        uint32_t key[RS_PER], rank[RS_PER];
-        const int64_t w0 = t0 + warp * (32 * RS_PER) + lane;
+        uint32_t rank[RS_PER], peers[RS_PER];
 #pragma unroll
-        for (int j = 0; j < RS_PER; ++j) key[j] = w0 + 32 * j < b ? src.key(w0 + 32 * j) : 0u;
+        for (int j = 0; j < RS_PER; ++j) {
+            uint32_t p = __ballot_sync(0xffffffffu, w0 + 32 * j < b);
+            for (int q = 0; q < bits; ++q) {
+                const bool one = key[j] >> (shift + q) & 1u;
+                const uint32_t v = __ballot_sync(0xffffffffu, one);
+                p &= one ? v : ~v;
+            }
+            peers[j] = p;
+        }
 #pragma unroll
         for (int j = 0; j < RS_PER; ++j) {
             const bool on = w0 + 32 * j < b;
-            const uint32_t dg = on ? (key[j] >> shift) & 255u : 256u;
-            const uint32_t peers = __match_any_sync(0xffffffffu, dg);
-            rank[j] = __popc(peers & ((1u << lane) - 1u));
-            if (on) rank[j] += cnt[warp][dg];
+            const uint32_t dg = (key[j] >> shift) & mask;
+            rank[j] = __popc(peers[j] & ((1u << lane) - 1u)) + (on ? cnt[warp][dg] : 0u);
             __syncwarp();
-            if (on && (peers >> lane) == 1u) cnt[warp][dg] += __popc(peers);    // the last of them
+            if (on && (peers[j] >> lane) == 1u) cnt[warp][dg] += __popc(peers[j]);    // the last of them
             __syncwarp();
         }
         __syncthreads();
@@ -155,9 +244,9 @@ radix_scatter_kernel(S src, int64_t N, int64_t span, int shift, const uint32_t* 
 #pragma unroll
         for (int j = 0; j < RS_PER; ++j)
             if (w0 + 32 * j < b) {
-                const uint32_t o = cnt[warp][(key[j] >> shift) & 255u] + rank[j];
+                const uint32_t o = cnt[warp][(key[j] >> shift) & mask] + rank[j];
                 ko[o] = key[j];
-                po[o] = src.pos(w0 + 32 * j);
+                po[o] = pos[j];
             }
         __syncthreads();
     }
@@ -168,8 +257,8 @@ radix_scatter_kernel(S src, int64_t N, int64_t span, int shift, const uint32_t* 
 // row's end comes after its tokens), and the list is cut into equal chunks: an entry costs
 // a read of D values, a row end a write of D values, so every chunk costs the same
 // whatever the tokens' distribution.  A row whose items lie in one chunk is written there.  A row
-// that is cut leaves its sums in `tail` (row goes on in the next chunk) and `head` (row
-// ends here, begun earlier); embed_join_kernel adds those in chunk order.
+// that is cut leaves its sums in carry rows: `tail` (the row goes on in the next chunk) and
+// `head` (it ends here, begun earlier); embed_join_kernel adds those in chunk order.
 struct Cut { int64_t r, i; };
 
 // Row ends and entries among the first d items, by a 33-way search of a full warp.  Row
@@ -243,31 +332,29 @@ __device__ __forceinline__ void store_row(T* __restrict__ row, int64_t c0, int64
     }
 }
 
-// carry rows hold a lane's E sums side by side: [slice][lane][E] floats
-template <int E>
+// carry rows are fp32 and padded to whole slices, so no column check
+template <int E, bool VEC>
 __device__ __forceinline__ void store_carry(float* __restrict__ p, int lane, const float (&acc)[E]) {
+    if constexpr (VEC) {
 #pragma unroll
-    for (int j = 0; j < E; j += 4)
-        *reinterpret_cast<float4*>(p + lane * E + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
-}
-template <int E>
-__device__ __forceinline__ void add_carry(const float* __restrict__ p, int lane, float (&acc)[E]) {
+        for (int j = 0; j < E; j += 4)
+            *reinterpret_cast<float4*>(p + lane * E + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+    } else {
 #pragma unroll
-    for (int j = 0; j < E; j += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(p + lane * E + j);
-        acc[j] += v.x; acc[j + 1] += v.y; acc[j + 2] += v.z; acc[j + 3] += v.w;
+        for (int j = 0; j < E; ++j) p[lane + 32 * j] = acc[j];
     }
 }
 
 constexpr int SG_WARPS = 4;
 constexpr int SG_UNROLL = 8;
 
-// head_row[chunk] = row that ends in this chunk but began earlier, else -1
+// head_row[chunk] = row that ends in this chunk but began earlier, else -1;
+// start[row] = chunk with the row's first entry, for rows that end in a later one
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(SG_WARPS * 32)
 embed_sum_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ pos, int64_t N, int64_t V,
                  int64_t D, int64_t chunk, const T* __restrict__ g, float scale, T* __restrict__ gw,
-                 float* __restrict__ carry, int64_t slices, int32_t* __restrict__ head_row) {
+                 float* __restrict__ carry, int64_t slices, int32_t* __restrict__ head_row, int32_t* __restrict__ start) {
     constexpr int E = Pack16<T>::E;
     constexpr int SLICE = 32 * E;
     __shared__ Cut cut[2];
@@ -283,7 +370,11 @@ embed_sum_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ 
     const int64_t r0 = cut[0].r, i0 = cut[0].i, r1 = cut[1].r;
     int64_t i1 = cut[1].i;
     const bool begun = r0 < V && i0 > 0 && (int64_t)key[i0 - 1] == r0;      // r0 has entries in earlier chunks
-    if (threadIdx.x == 0 && blockIdx.y == 0) head_row[c] = begun && r1 > r0 ? (int32_t)r0 : -1;
+    const bool open = r1 < V && i1 > i0 && (int64_t)key[i1 - 1] == r1;      // r1 goes on in the next one
+    if (threadIdx.x == 0 && blockIdx.y == 0) {
+        head_row[c] = begun && r1 > r0 ? (int32_t)r0 : -1;
+        if (open && !(begun && r1 == r0)) start[r1] = (int32_t)c;
+    }
     if (r1 == V) {                      // what follows the last row's end has no gradient
         while (i1 > i0 && (int64_t)key[i1 - 1] >= V) --i1;
     }
@@ -297,7 +388,7 @@ embed_sum_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ 
         int64_t r = r0;
         auto end_rows = [&](int64_t upto) {                 // rows r .. upto-1 end here
             for (; r < upto; ++r) {
-                if (r == r0 && begun) store_carry<E>(head, lane, acc);
+                if (r == r0 && begun) store_carry<E, VEC>(head, lane, acc);
                 else store_row<T, VEC>(gw + r * D, c0, D, lane, scale, acc);
 #pragma unroll
                 for (int j = 0; j < E; ++j) acc[j] = 0.0f;
@@ -319,49 +410,85 @@ embed_sum_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ 
             }
         }
         end_rows(r1);
-        if (r1 < V) store_carry<E>(tail, lane, acc);        // all zeros when r1 has no entry here
+        if (open) store_carry<E, VEC>(tail, lane, acc);
     }
 }
 
-// One warp = one cut row x one slice: tails from the row's first chunk on, then the head.
+// One CTA = one cut row x a share of its groups of 128 columns.  Short rows: a warp per
+// group adds the row's tails, then its head.  Long ones (a frequent token's row is cut into
+// hundreds of chunks): the CTA's warps take equal runs of the tails, joined in shared memory.
+constexpr int JN_WARPS = 8;
+constexpr int JN_SHORT = 8;
+
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(SG_WARPS * 32)
-embed_join_kernel(const uint32_t* __restrict__ key, int64_t N, int64_t V, int64_t D, int64_t chunk,
-                  int64_t nchunk, float scale, T* __restrict__ gw, const float* __restrict__ carry,
-                  int64_t slices, const int32_t* __restrict__ head_row) {
-    constexpr int E = Pack16<T>::E;
-    constexpr int SLICE = 32 * E;
+__global__ void __launch_bounds__(JN_WARPS * 32)
+embed_join_kernel(int64_t D, float scale, T* __restrict__ gw, const float* __restrict__ carry, int64_t ldc,
+                  const int32_t* __restrict__ head_row, const int32_t* __restrict__ start) {
+    __shared__ float4 part[JN_WARPS][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t c = blockIdx.x;
     const int64_t r = head_row[c];
     if (r < 0) return;
-    // the row's first entry: the number of entries with a smaller token (33-way search)
-    int64_t lo = 0, hi = N;
-    while (lo < hi) {
-        const int64_t step = (hi - lo + 32) / 33;
-        const int64_t m = lo + step * (lane + 1) - 1;
-        const int n = __popc(__ballot_sync(0xffffffffu, m < hi && (int64_t)key[m] < r));
-        const int64_t nlo = lo + step * n;
-        hi = n == 32 ? hi : (nlo + step - 1 < hi ? nlo + step - 1 : hi);
-        lo = nlo;
-    }
-    const int64_t first = (lo + r) / chunk;                 // r row ends come before it
-    for (int64_t s = (int64_t)blockIdx.y * SG_WARPS + warp; s < slices; s += (int64_t)gridDim.y * SG_WARPS) {
-        float acc[E];
+    const int64_t first = start[r], n = c - first;
+    const int64_t groups = ldc / 128;
+    auto sum = [&](int64_t g, int64_t a, int64_t b) {           // tails of chunks first+a .. first+b-1
+        const float4* p = reinterpret_cast<const float4*>(carry + (2 * (first + a) + 1) * ldc + g * 128) + lane;
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+        int64_t q = a;
+        for (; q + 8 <= b; q += 8) {
+            float4 v[8];
 #pragma unroll
-        for (int j = 0; j < E; ++j) acc[j] = 0.0f;
-#pragma unroll 8
-        for (int64_t q = first; q < c; ++q) add_carry<E>(carry + ((2 * q + 1) * slices + s) * SLICE, lane, acc);
-        add_carry<E>(carry + ((2 * c) * slices + s) * SLICE, lane, acc);
-        store_row<T, VEC>(gw + r * D, s * SLICE, D, lane, scale, acc);
+            for (int u = 0; u < 8; ++u) v[u] = __ldg(p + (int64_t)u * (ldc / 2));
+            p += 8 * (ldc / 2);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) { s.x += v[u].x; s.y += v[u].y; s.z += v[u].z; s.w += v[u].w; }
+        }
+        for (; q < b; ++q, p += ldc / 2) {
+            const float4 v = __ldg(p);
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        }
+        return s;
+    };
+    auto finish = [&](int64_t g, float4 s) {
+        const float4 h = *(reinterpret_cast<const float4*>(carry + 2 * c * ldc + g * 128) + lane);
+        const float v[4] = {(s.x + h.x) * scale, (s.y + h.y) * scale, (s.z + h.z) * scale, (s.w + h.w) * scale};
+        const int64_t col = g * 128 + lane * 4;
+        T* o = gw + r * D + col;
+        if (VEC && col + 4 <= D) {
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+            else *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(v), pack2<T>(v + 2));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (col + j < D) o[j] = from_f32<T>(v[j]);
+        }
+    };
+    if (n <= JN_SHORT) {
+        for (int64_t g = (int64_t)blockIdx.y * JN_WARPS + warp; g < groups; g += (int64_t)gridDim.y * JN_WARPS)
+            finish(g, sum(g, 0, n));
+        return;
+    }
+    for (int64_t g = blockIdx.y; g < groups; g += gridDim.y) {
+        part[warp][lane] = sum(g, n * warp / JN_WARPS, n * (warp + 1) / JN_WARPS);
+        __syncthreads();
+        if (warp == 0) {
+            float4 s = part[0][lane];
+#pragma unroll
+            for (int w = 1; w < JN_WARPS; ++w) {
+                const float4 v = part[w][lane];
+                s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+            }
+            finish(g, s);
+        }
+        __syncthreads();
     }
 }
 
 // ------------------------------------------------------------------- plans
 struct EmbedPlan {
-    int64_t keys_at, hist_at, head_at, carry_at, bytes;
+    int64_t hist_at, head_at, start_at, carry_at, bytes;
     int64_t chunk, nchunk, slices, tiles;
-    int passes;
+    int passes, bits;
 };
 
 static int bits_of(uint64_t v) { int n = 0; while (v) { ++n; v >>= 1; } return n; }
@@ -369,15 +496,19 @@ static int bits_of(uint64_t v) { int n = 0; while (v) { ++n; v >>= 1; } return n
 static EmbedPlan embed_plan(int64_t N, int64_t V, int64_t D, int es) {
     EmbedPlan p;
     auto up = [](int64_t v) { return cdiv(v, 256) * 256; };
-    p.tiles = N > 0 ? cdiv(N, rs_span(N)) : 0;
-    p.passes = (int)cdiv(bits_of((uint64_t)V), 8);          // keys 0 .. V
+    p.tiles = N > RK_MAX ? cdiv(N, rs_span(N)) : 0;
+    const int bits = bits_of((uint64_t)V);                  // keys 0 .. V
+    p.passes = (bits + RS_BITS - 1) / RS_BITS;
+    p.bits = (bits + p.passes - 1) / p.passes;
     p.slices = cdiv(D * es, 512);                           // 32 lanes x 16 bytes
-    p.chunk = 64;
+    // about 16 chunks per SM, between 16 items (a chunk costs two searches) and 128
+    p.chunk = 16;
+    while (p.chunk < 128 && (V + N) / p.chunk > 148 * 16) p.chunk *= 2;
     p.nchunk = cdiv(V + N, p.chunk);
-    p.keys_at = 0;
-    p.hist_at = p.keys_at + up(4 * 4 * N);
+    p.hist_at = up(4 * 4 * N);                              // two (token, position) buffers
     p.head_at = p.hist_at + up(p.tiles * RS_BINS * 4);
-    p.carry_at = p.head_at + up(p.nchunk * 4);
+    p.start_at = p.head_at + up(p.nchunk * 4);
+    p.carry_at = p.start_at + up(V * 4);
     p.bytes = p.carry_at + p.nchunk * 2 * p.slices * (512 / es) * 4;
     return p;
 }
@@ -395,33 +526,41 @@ static int check_embed(int64_t N, int64_t V, int64_t D, int ids64, int dtype, co
 template <typename T, typename I>
 static void embed_fwd_launch(const I* ids, int64_t N, const T* w, int64_t V, int64_t D, float scale, T* y,
                              cudaStream_t st) {
-    const int64_t vecs = cdiv(N * D, Pack16<T>::E);
+    constexpr int E = Pack16<T>::E;
+    const int64_t vecs = cdiv(N * D, E);
     const unsigned grid = (unsigned)cdiv(vecs, EM_THREADS * EM_UNROLL);
-    if (D % Pack16<T>::E == 0 && aligned16(w))
-        embed_fwd_kernel<T, I, true><<<grid, EM_THREADS, 0, st>>>(ids, N, w, V, D, scale, y);
+    if (D % E || !aligned16(w))
+        embed_fwd_kernel<T, I, int64_t, false><<<grid, EM_THREADS, 0, st>>>(ids, N, w, V, D, 0, scale, y);
+    else if (vecs + EM_THREADS * EM_UNROLL < (1ll << 32))
+        embed_fwd_kernel<T, I, uint32_t, true><<<grid, EM_THREADS, 0, st>>>(ids, N, w, V, D, (uint32_t)(D / E), scale, y);
     else
-        embed_fwd_kernel<T, I, false><<<grid, EM_THREADS, 0, st>>>(ids, N, w, V, D, scale, y);
+        embed_fwd_kernel<T, I, int64_t, true><<<grid, EM_THREADS, 0, st>>>(ids, N, w, V, D, D / E, scale, y);
 }
 
+// sorted tokens, followed by their positions (at + N)
 template <typename I>
 static const uint32_t* embed_sort(const I* ids, int64_t N, int64_t V, int64_t pad, const EmbedPlan& p, char* ws,
                                   cudaStream_t st) {
-    uint32_t* buf[2] = {reinterpret_cast<uint32_t*>(ws + p.keys_at),
-                        reinterpret_cast<uint32_t*>(ws + p.keys_at) + 2 * N};
+    uint32_t* buf[2] = {reinterpret_cast<uint32_t*>(ws), reinterpret_cast<uint32_t*>(ws) + 2 * N};
+    const KeysOfIds<I> in{ids, V, pad};
+    if (N <= RK_MAX) {
+        rank_sort_kernel<I><<<(unsigned)cdiv(N, 32), RK_THREADS, 0, st>>>(in, (int)N, buf[0], buf[0] + N);
+        return buf[0];
+    }
     uint32_t* hist = reinterpret_cast<uint32_t*>(ws + p.hist_at);
     const int64_t span = rs_span(N);
-    const KeysOfIds<I> in{ids, V, pad};
+    const unsigned grid = (unsigned)p.tiles;
+    const uint32_t mask = (1u << p.bits) - 1u;
     uint32_t* src = nullptr;
     for (int q = 0; q < p.passes; ++q) {
         uint32_t* dst = buf[q & 1];
-        const unsigned grid = (unsigned)p.tiles;
         if (q == 0) {
-            radix_count_kernel<<<grid, RS_THREADS, 0, st>>>(in, N, span, 0, hist);
-            radix_scatter_kernel<<<grid, RS_THREADS, 0, st>>>(in, N, span, 0, hist, dst, dst + N);
+            radix_count_kernel<<<grid, RS_THREADS, 0, st>>>(in, N, span, 0, mask, hist);
+            radix_scatter_kernel<<<grid, RS_THREADS, 0, st>>>(in, N, span, 0, p.bits, hist, dst, dst + N);
         } else {
             const KeysOfPairs pairs{src, src + N};
-            radix_count_kernel<<<grid, RS_THREADS, 0, st>>>(pairs, N, span, 8 * q, hist);
-            radix_scatter_kernel<<<grid, RS_THREADS, 0, st>>>(pairs, N, span, 8 * q, hist, dst, dst + N);
+            radix_count_kernel<<<grid, RS_THREADS, 0, st>>>(pairs, N, span, p.bits * q, mask, hist);
+            radix_scatter_kernel<<<grid, RS_THREADS, 0, st>>>(pairs, N, span, p.bits * q, p.bits, hist, dst, dst + N);
         }
         src = dst;
     }
@@ -431,19 +570,21 @@ static const uint32_t* embed_sort(const I* ids, int64_t N, int64_t V, int64_t pa
 template <typename T>
 static void embed_bwd_launch(const uint32_t* key, int64_t N, int64_t V, int64_t D, const T* g, float scale, T* gw,
                              const EmbedPlan& p, char* ws, cudaStream_t st) {
+    constexpr int E = Pack16<T>::E;
     float* carry = reinterpret_cast<float*>(ws + p.carry_at);
     int32_t* head = reinterpret_cast<int32_t*>(ws + p.head_at);
-    const uint32_t* pos = key + N;
+    int32_t* start = reinterpret_cast<int32_t*>(ws + p.start_at);
     const dim3 grid((unsigned)p.nchunk, (unsigned)std::min<int64_t>(cdiv(p.slices, SG_WARPS), 65535));
+    const int64_t ldc = p.slices * 32 * E;
+    const dim3 jgrid((unsigned)p.nchunk, (unsigned)std::min<int64_t>(cdiv(ldc, 256), 4));
     auto go = [&](auto vec) {
         constexpr bool VEC = decltype(vec)::value;
-        embed_sum_kernel<T, VEC><<<grid, SG_WARPS * 32, 0, st>>>(key, pos, N, V, D, p.chunk, g, scale, gw, carry,
-                                                                 p.slices, head);
+        embed_sum_kernel<T, VEC><<<grid, SG_WARPS * 32, 0, st>>>(key, key + N, N, V, D, p.chunk, g, scale, gw, carry,
+                                                                 p.slices, head, start);
         if (N > 0)
-            embed_join_kernel<T, VEC><<<grid, SG_WARPS * 32, 0, st>>>(key, N, V, D, p.chunk, p.nchunk, scale, gw,
-                                                                      carry, p.slices, head);
+            embed_join_kernel<T, VEC><<<jgrid, JN_WARPS * 32, 0, st>>>(D, scale, gw, carry, ldc, head, start);
     };
-    if (D % Pack16<T>::E == 0 && aligned16(g) && aligned16(gw)) go(std::true_type{});
+    if (D % E == 0 && aligned16(g) && aligned16(gw)) go(std::true_type{});
     else go(std::false_type{});
 }
 

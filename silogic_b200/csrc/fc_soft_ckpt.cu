@@ -13,20 +13,57 @@
 
 namespace slg {
 
-// byte j of a code word as a float: 2^23 + q has q in its low mantissa bits
-__device__ __forceinline__ float code_f32(uint32_t word, int j) {
-    return __uint_as_float(__byte_perm(word, 0x4b000000u, 0x7540u + j)) - 8388608.0f;
+// Two fp32 values in one 64-bit register: the packed instructions do two samples an issue
+// slot, and issue slots bound the scalar form of this kernel (72% busy, L2 at 53%).
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
 }
-// twice byte j, from 2^24 + 2 q: another expression than code_f32's, so that the second use
-// of a word decodes it again instead of keeping 64 decoded values in registers
-__device__ __forceinline__ float code2_f32(uint32_t word, int j) {
-    return __uint_as_float(__byte_perm(word, 0x4b800000u, 0x7640u + j)) - 16777216.0f;
+__device__ __forceinline__ void unpair(f32x2 p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 
+// bytes j and j + 1 of a code word as floats: 2^23 + q has q in its low mantissa bits
+__device__ __forceinline__ f32x2 codes_f32(uint32_t word, int j) {
+    const f32x2 raw = pair(__uint_as_float(__byte_perm(word, 0x4b000000u, 0x7540u + j)),
+                           __uint_as_float(__byte_perm(word, 0x4b000000u, 0x7541u + j)));
+    return add2(raw, pair(-8388608.0f, -8388608.0f));
+}
+// twice bytes j and j + 1, from 2^24 + 2 q: another expression than codes_f32's, so that the
+// second use of a word decodes it again instead of keeping 64 decoded values in registers
+__device__ __forceinline__ f32x2 codes2_f32(uint32_t word, int j) {
+    const f32x2 raw = pair(__uint_as_float(__byte_perm(word, 0x4b800000u, 0x7640u + j)),
+                           __uint_as_float(__byte_perm(word, 0x4b800000u, 0x7641u + j)));
+    return add2(raw, pair(-16777216.0f, -16777216.0f));
+}
+
+// One candidate of a node: its rows and weight, and per block of the chunk (w step, w lo)
+// and (step / 2, lo).  Places past K have weight and bounds 0 and read row 0.
+struct alignas(16) CkptCand {
+    const uint32_t* codes;
+    float4* gx;
+};
 template <int NODE, int KT>
 struct CkptSmem {
     FcSmem<NODE, 2> node;
-    float4 b[FS_ITER][2 * KT];      // w step, w lo, step, lo of a candidate's block
+    CkptCand row[2 * KT];
+    float2 mix[FS_ITER][2 * KT];    // w step, w
+    float2 back[FS_ITER][2 * KT];   // step / 2, lo
     float c[FS_ITER][2];            // sum_k w lo
 };
 
@@ -57,25 +94,28 @@ fc_soft_bwd_ckpt_kernel(const uint32_t* __restrict__ codes, uint32_t ldw, const 
     }
     CkptSmem<NODE, KT>& S = smem[warp];
     stage_node<NODE, 2>(S.node, o, cand, conn, K, conn_ste, params, np_stride, gate_hard, inv_tau, lane);
-    // slot j's candidate k sits at j KT + k; unused places have weight and bounds 0 and read row 0
     for (int e = lane; e < EK * FS_ITER; e += 32) {
         const int it = e % FS_ITER, p = e / FS_ITER, j = p / KT, k = p % KT;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        float2 mix = make_float2(0.f, 0.f), back = mix;
         const int64_t blk = chunk * FS_ITER + it;
+        const int64_t row = k < K ? S.node.cand[j * K + k] : 0;
         if (k < K && blk < nblk) {
-            const float2 b = __ldg(&bounds[(int64_t)S.node.cand[j * K + k] * nblk + blk]);
+            const float2 b = __ldg(&bounds[row * nblk + blk]);
             const float w = S.node.w[j * K + k];
-            v = make_float4(w * b.y, w * b.x, b.y, b.x);
+            mix = make_float2(w * b.y, w);
+            back = make_float2(0.5f * b.y, b.x);
         }
-        S.b[it][p] = v;
+        S.mix[it][p] = mix;
+        S.back[it][p] = back;
+        if (it == 0) S.row[p] = {codes + row * ldw, gx ? gx + row * nv : nullptr};
     }
     __syncwarp();
     if (lane < 2 * FS_ITER) {
+        const int it = lane >> 1, j = lane & 1;
         float c = 0.0f;
-        for (int k = 0; k < K; ++k) c += S.b[lane >> 1][(lane & 1) * KT + k].y;
-        S.c[lane >> 1][lane & 1] = c;
+        for (int k = 0; k < KT; ++k) c += S.mix[it][j * KT + k].y * S.back[it][j * KT + k].y;
+        S.c[it][j] = c;
     }
-    __syncwarp();
     float acc_node[NPG], acc_w[EK];
 #pragma unroll
     for (int q = 0; q < NPG; ++q) acc_node[q] = 0.0f;
@@ -90,22 +130,22 @@ fc_soft_bwd_ckpt_kernel(const uint32_t* __restrict__ codes, uint32_t ldw, const 
         const bool on = v < nv;
         uint32_t q[EK];
 #pragma unroll
-        for (int e = 0; e < EK; ++e)
-            q[e] = on && (KT == 1 || e % KT < K)
-                       ? __ldg(codes + (size_t)(uint32_t)S.node.cand[(e / KT) * K + e % KT] * ldw + v) : 0u;
+        for (int e = 0; e < EK; ++e) q[e] = on ? __ldg(S.row[e].codes + v) : 0u;
         const float4 g = on ? gy[o * nv + v] : make_float4(0.f, 0.f, 0.f, 0.f);
         float a[4][2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const float c = S.c[it][j];
-#pragma unroll
-            for (int s = 0; s < 4; ++s) a[s][j] = c;
+            f32x2 a01 = pair(c, c), a23 = a01;
 #pragma unroll
             for (int k = 0; k < KT; ++k) {
-                const float wstep = S.b[it][j * KT + k].x;
-#pragma unroll
-                for (int s = 0; s < 4; ++s) a[s][j] = fmaf(wstep, code_f32(q[j * KT + k], s), a[s][j]);
+                const float w = S.mix[it][j * KT + k].x;
+                const f32x2 ww = pair(w, w);
+                a01 = fma2(ww, codes_f32(q[j * KT + k], 0), a01);
+                a23 = fma2(ww, codes_f32(q[j * KT + k], 2), a23);
             }
+            unpair(a01, a[0][j], a[1][j]);
+            unpair(a23, a[2][j], a[3][j]);
         }
         const float gs[4] = {g.x, g.y, g.z, g.w};
         float ga[4][2];
@@ -113,22 +153,26 @@ fc_soft_bwd_ckpt_kernel(const uint32_t* __restrict__ codes, uint32_t ldw, const 
         for (int s = 0; s < 4; ++s) node_bwd<NODE, 2>(S.node.np, a[s], gs[s], ga[s], acc_node);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
+            const f32x2 g01 = pair(ga[0][j], ga[1][j]), g23 = pair(ga[2][j], ga[3][j]);
             const float sum = (ga[0][j] + ga[1][j]) + (ga[2][j] + ga[3][j]);
 #pragma unroll
             for (int k = 0; k < KT; ++k) {
-                if (KT > 1 && k >= K) break;
                 const int e = j * KT + k;
                 if (KT > 1) {
-                    float t = 0.0f;
-#pragma unroll
-                    for (int s = 0; s < 4; ++s) t = fmaf(ga[s][j], code2_f32(q[e], s), t);
-                    const float4 b = S.b[it][e];
-                    acc_w[e] = fmaf(0.5f * b.z, t, fmaf(b.w, sum, acc_w[e]));
+                    const f32x2 t = fma2(g01, codes2_f32(q[e], 0), mul2(g23, codes2_f32(q[e], 2)));
+                    float t0, t1;
+                    unpair(t, t0, t1);
+                    const float2 b = S.back[it][e];
+                    acc_w[e] = fmaf(b.x, t0 + t1, fmaf(b.y, sum, acc_w[e]));
                 }
-                const float w = S.node.w[j * K + k];
-                if (gx && on && w != 0.0f)
-                    atomicAdd(&gx[(int64_t)S.node.cand[j * K + k] * nv + v],
-                              make_float4(ga[0][j] * w, ga[1][j] * w, ga[2][j] * w, ga[3][j] * w));
+                const float w = S.mix[it][e].y;
+                if (w != 0.0f && gx && on) {
+                    const f32x2 ww = pair(w, w);
+                    float4 r;
+                    unpair(mul2(g01, ww), r.x, r.y);
+                    unpair(mul2(g23, ww), r.z, r.w);
+                    atomicAdd(S.row[e].gx + v, r);
+                }
             }
         }
     }
