@@ -168,12 +168,22 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
                         if (lane == __ffs(__ballot_sync(0xffffffffu, t == reach)) - 1) t = 0;
                     }
                 }
+                const float least = reach ? unordered(reach) : -CUDART_INF_F;
+                uint32_t left = 0;
 #pragma unroll
-                for (int i = 0; i < BM_PER; ++i) {
-                    uint32_t in = __ballot_sync(0xffffffffu, (valid >> i & 1u) && ordered(x[i]) >= reach);
-                    if (in == 0) continue;
-                    const uint64_t k = cand_key(x[i], (uint32_t)(base + (i / E) * 32 * E + i % E));
-                    for (; in; in &= in - 1) {
+                for (int i = 0; i < BM_PER; ++i) left |= x[i] >= least ? 1u << i : 0u;
+                left &= valid;
+                // the few that qualify are read again (from L1) and inserted one by one: short
+                // code, because a step of few beams mostly waits for instructions
+                while (__any_sync(0xffffffffu, left != 0)) {
+                    uint64_t k = 0;
+                    if (left) {
+                        const int i = __ffs(left) - 1;
+                        left &= left - 1;
+                        const int64_t at = base + (i / E) * 32 * E + i % E;
+                        k = cand_key(clean(to_f32(row[at])), (uint32_t)at);
+                    }
+                    for (uint32_t in = __ballot_sync(0xffffffffu, k > bar); in; in &= in - 1) {
                         const uint64_t w = __shfl_sync(0xffffffffu, k, __ffs(in) - 1);
                         if (w <= bar) continue;
                         const int at = __popc(__ballot_sync(0xffffffffu, lane < width && list > w));
@@ -259,9 +269,10 @@ static cudaError_t beam_step_launch(const T* x, int64_t B, int beams, int64_t V,
                                     const uint8_t* finished, int32_t eos, int width, float* out_scores, int64_t* parents,
                                     int64_t* tokens, uint8_t* out_finished, cudaStream_t st) {
     const int units = (int)cdiv(V, BM_UNIT);
-    // CTAs per entry: as many as have a unit for every warp, at most 8, no more than fill the GPU
+    // CTAs per entry: as many as have a unit for every warp, at most 8, and all resident at
+    // once (two per SM): a second wave of clusters would start after the first one's joins
     int cs = 1;
-    while (cs < 8 && (int64_t)cs * BM_WARPS < (int64_t)beams * units && B * cs < 2 * sm_count()) cs *= 2;
+    while (cs < 8 && (int64_t)cs * BM_WARPS < (int64_t)beams * units && B * cs * 2 <= 2 * sm_count()) cs *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(B * cs));
     cfg.blockDim = dim3(BM_THREADS);
@@ -312,23 +323,46 @@ reorder_features_kernel(const float* __restrict__ in, int64_t F, int64_t ldi, in
         out[f * ldo + r] = on ? __ldg(&in[f * ldi + src]) : 0.0f;
 }
 
-// The same on bits: a warp builds one 32-sample word of a row by ballot, for many rows.
-constexpr int RP_WARPS = 8;
-__global__ void __launch_bounds__(RP_WARPS * 32)
+// The same on bits.  A thread builds one 32-bit word of a row bit by bit; a CTA's threads
+// walk (row, word) of 32 word columns, row by row, so stores are whole lines (a warp that
+// built one word by ballot stored 4 bytes at a time: 10 us instead of 4 on 10,000 x 512).
+// The sources of the 1,024 samples are worked out once per CTA.
+constexpr int RP_THREADS = 256;
+constexpr int RP_WORDS = 32;
+constexpr int RP_PER = 2;               // words per thread
+__global__ void __launch_bounds__(RP_THREADS)
 reorder_packed_kernel(const uint32_t* __restrict__ in, int64_t F, int64_t ldi, int64_t n,
                       const int64_t* __restrict__ parents, int beams, int width, uint32_t* __restrict__ out,
                       int64_t ldo) {
-    const int lane = threadIdx.x & 31;
-    const int64_t w = blockIdx.x;                           // 32-bit word of the output rows
-    const int64_t r = w * 32 + lane;
-    const bool on = r < n;
-    const int64_t src = on ? beam_source(parents, (uint32_t)r, beams, width) : 0;
-    const uint32_t bit = (uint32_t)src & 31u;
-    in += src >> 5;
+    __shared__ int64_t word_of[RP_WORDS];       // first source word of an output word
+    __shared__ uint16_t from[RP_WORDS][34];     // bit's source: 32 (word - first) + bit, 0xffff: none
+    const int64_t w0 = (int64_t)blockIdx.y * RP_WORDS;
+    const int words = (int)min((int64_t)RP_WORDS, ldo - w0);
+    for (int i = threadIdx.x; i < words * 32; i += RP_THREADS) {
+        // an output word's 32 samples span at most 32 / width + 2 entries of at most 32
+        // beams: their sources lie within 32 * 34 samples after the first entry's
+        const int64_t r0 = (w0 + i / 32) * 32, r = r0 + i % 32;
+        const int64_t first = (r0 / width * beams) >> 5;
+        from[i / 32][i % 32] =
+            r < n ? (uint16_t)(beam_source(parents, (uint32_t)r, beams, width) - first * 32) : (uint16_t)0xffff;
+        if (i % 32 == 0) word_of[i / 32] = first;
+    }
+    __syncthreads();
+    const int64_t total = F * words;
+#pragma unroll
+    for (int u = 0; u < RP_PER; ++u) {
+        const int64_t t = ((int64_t)blockIdx.x * RP_PER + u) * RP_THREADS + threadIdx.x;
+        if (t >= total) continue;
+        const int64_t f = total < (1ll << 32) ? (int64_t)((uint32_t)t / (uint32_t)words) : t / words;
+        const int w = (int)(t - f * words);
+        const uint32_t* src = in + f * ldi + word_of[w];
+        uint32_t bits = 0;
 #pragma unroll 8
-    for (int64_t f = (int64_t)blockIdx.y * RP_WARPS + (threadIdx.x >> 5); f < F; f += (int64_t)gridDim.y * RP_WARPS) {
-        const uint32_t word = __ballot_sync(0xffffffffu, on && (__ldg(&in[f * ldi]) >> bit & 1u));
-        if (lane == 0) out[f * ldo + w] = word;
+        for (int j = 0; j < 32; ++j) {
+            const uint32_t s = from[w][j];
+            if (s != 0xffffu) bits |= (__ldg(src + (s >> 5)) >> (s & 31u) & 1u) << j;
+        }
+        out[f * ldo + w0 + w] = bits;
     }
 }
 
@@ -412,9 +446,11 @@ extern "C" int slg_beam_reorder_packed(const uint64_t* in, int64_t F, int64_t ld
     if (st) return st;
     if (F < 0 || ldi * 64 < B * beams || ldo * 64 < B * width)
         return set_error(SLG_ERR_ARG, "slg_beam_reorder_packed: bad sizes");
-    const dim3 grid((unsigned)(2 * ldo), (unsigned)std::min<int64_t>(cdiv(F, RP_WARPS * 8), 65535));
-    reorder_packed_kernel<<<grid, RP_WARPS * 32, 0, as_stream(stream)>>>(reinterpret_cast<const uint32_t*>(in), F, 2 * ldi,
-                                                               B * width, parents, beams, width,
-                                                               reinterpret_cast<uint32_t*>(out), 2 * ldo);
+    const int64_t per_row = std::min<int64_t>(2 * ldo, RP_WORDS), tiles = cdiv(2 * ldo, RP_WORDS);
+    if (tiles > 65535) return set_error(SLG_ERR_ARG, "slg_beam_reorder_packed: batch too large");
+    const dim3 grid((unsigned)cdiv(F * per_row, RP_THREADS * RP_PER), (unsigned)tiles);
+    reorder_packed_kernel<<<grid, RP_THREADS, 0, as_stream(stream)>>>(reinterpret_cast<const uint32_t*>(in), F, 2 * ldi,
+                                                                     B * width, parents, beams, width,
+                                                                     reinterpret_cast<uint32_t*>(out), 2 * ldo);
     return check_launch("slg_beam_reorder_packed");
 }

@@ -189,71 +189,100 @@ __device__ __forceinline__ void node_bwd(const float* __restrict__ np, const flo
 }
 
 // ----------------------------------------------------- parameter staging
-// Transform one node's raw parameters into np[] (see header).  Executed by one
-// warp cooperatively; `raw` = node parameter row.  gate_hard: STE one-hot gate
-// in the forward value.  Returns after __syncwarp.
+// A warp stages one node before it walks the batch, so this is pure latency: values are
+// loaded one per lane (`first` = the lane's raw[lane], loaded early by the caller), every
+// exponential is taken by its own lane, and sums run over the lanes' values in index order
+// by shuffles -- the order, and so the bits, of a serial loop.
+
+// Transform one node's raw parameters into np[] (see header).  Executed by one warp
+// cooperatively; `raw` = node parameter row.  gate_hard: STE one-hot gate in the forward
+// value.  Returns after __syncwarp.
 template <int NODE, int AR>
-__device__ __forceinline__ void stage_node_params(const float* __restrict__ raw, float* np, int gate_hard,
+__device__ __forceinline__ float node_param_first(const float* __restrict__ raw, int lane) {
+    constexpr int N = NODE == N_GATE16 ? 16 : NodeSize<NODE, AR>::NPG;
+    return lane < N ? raw[lane] : 0.0f;
+}
+
+template <int NODE, int AR>
+__device__ __forceinline__ void stage_node_params(const float* __restrict__ raw, float first, float* np, int gate_hard,
                                                   float inv_tau, int lane) {
     constexpr int P = 1 << AR;
+    constexpr unsigned FULL = 0xffffffffu;
     if constexpr (NODE == N_GATE16) {
-        if (lane == 0) {
-            float mx = raw[0];
-            int arg = 0;
-            for (int i = 1; i < 16; ++i)
-                if (raw[i] > mx) { mx = raw[i]; arg = i; }
-            float e[16], s = 0.0f;
-            for (int i = 0; i < 16; ++i) { e[i] = expf(raw[i] - mx); s += e[i]; }
-            for (int c = 0; c < 4; ++c) {
-                float v = 0.0f;
-                if (gate_hard) v = c_basis[arg][c];
-                else
-                    for (int i = 0; i < 16; ++i) v += (e[i] / s) * c_basis[i][c];
-                np[c] = v;
-            }
+        float mx = __shfl_sync(FULL, first, 0);
+        int arg = 0;
+#pragma unroll
+        for (int i = 1; i < 16; ++i) {
+            const float r = __shfl_sync(FULL, first, i);
+            if (r > mx) { mx = r; arg = i; }
         }
+        const float e = expf(first - mx);
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s += __shfl_sync(FULL, e, i);
+        const float prob = e / s;
+        const int c = lane & 3;
+        float v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v += __shfl_sync(FULL, prob, i) * c_basis[i][c];
+        if (lane < 4) np[lane] = gate_hard ? c_basis[arg][c] : v;
     } else if constexpr (NODE == N_COEF) {
-        if (lane < 4) np[lane] = raw[lane];
+        if (lane < 4) np[lane] = first;
     } else if constexpr (NODE == N_COEF_SIG) {
-        if (lane < 4) np[lane] = raw[lane];
+        if (lane < 4) np[lane] = first;
         if (lane == 0) np[4] = inv_tau;
     } else if constexpr (NODE == N_HYBRID_S) {
-        for (int q = lane; q < P; q += 32) np[q] = raw[q];
+        for (int q = lane; q < P; q += 32) np[q] = q == lane ? first : raw[q];
     } else if constexpr (NODE == N_WALSH) {
-        for (int q = lane; q < P; q += 32) np[q] = raw[q];
+        for (int q = lane; q < P; q += 32) np[q] = q == lane ? first : raw[q];
         if (lane == 0) np[P] = inv_tau;
     } else if constexpr (NODE == N_MULTI || NODE == N_HYBRID) {
-        for (int q = lane; q < P; q += 32) np[q] = sigmoidf_(raw[q]);
+        for (int q = lane; q < P; q += 32) np[q] = sigmoidf_(q == lane ? first : raw[q]);
     } else {
-        for (int q = lane; q <= AR; q += 32) np[q] = raw[q];
+        if (lane <= AR) np[lane] = first;
     }
     __syncwarp();
 }
 
-// Connection weights of one node: softmax over K per slot (one-hot when ste == 1; the
+template <int NODE, int AR>
+__device__ __forceinline__ void stage_node_params(const float* __restrict__ raw, float* np, int gate_hard,
+                                                  float inv_tau, int lane) {
+    stage_node_params<NODE, AR>(raw, node_param_first<NODE, AR>(raw, lane), np, gate_hard, inv_tau, lane);
+}
+
+// Connection weights of one node: softmax over K (<= 16) per slot (one-hot when ste == 1; the
 // values as given when ste == 2, i.e. already-normalised weights).
-// w[j*K + k]; executed by lanes j < AR.
-__device__ __forceinline__ void stage_conn(const float* __restrict__ logits, float* w, int AR, int K,
+// w[j*K + k]; lanes take whole slots, 32 / K at a time.
+__device__ __forceinline__ void stage_conn(const float* __restrict__ logits, float first, float* w, int AR, int K,
                                            int ste, int lane) {
+    constexpr unsigned FULL = 0xffffffffu;
     if (ste == 2) {
-        for (int e = lane; e < AR * K; e += 32) w[e] = logits[e];
+        for (int e = lane; e < AR * K; e += 32) w[e] = e == lane ? first : logits[e];
         __syncwarp();
         return;
     }
-    if (lane < AR) {
-        const float* l = logits + lane * K;
-        float mx = l[0];
+    const int per = 32 / K, slot = lane / K, k = lane - slot * K, base = slot < per ? slot * K : 0;
+    for (int j0 = 0; j0 < AR; j0 += per) {
+        const int e = j0 * K + lane;
+        const bool on = slot < per && j0 + slot < AR;
+        const float l = !on ? 0.0f : j0 == 0 ? first : logits[e];
+        float mx = __shfl_sync(FULL, l, base);
         int arg = 0;
-        for (int k = 1; k < K; ++k)
-            if (l[k] > mx) { mx = l[k]; arg = k; }
-        if (ste) {
-            for (int k = 0; k < K; ++k) w[lane * K + k] = (k == arg) ? 1.0f : 0.0f;
-        } else {
-            float s = 0.0f;
-            for (int k = 0; k < K; ++k) s += expf(l[k] - mx);
-            const float inv = 1.0f / s;
-            for (int k = 0; k < K; ++k) w[lane * K + k] = expf(l[k] - mx) * inv;
+#pragma unroll 4
+        for (int i = 1; i < K; ++i) {
+            const float r = __shfl_sync(FULL, l, base + i);
+            if (r > mx) { mx = r; arg = i; }
         }
+        float v;
+        if (ste) v = k == arg ? 1.0f : 0.0f;
+        else {
+            const float x = expf(l - mx);
+            float s = 0.0f;
+#pragma unroll 4
+            for (int i = 0; i < K; ++i) s += __shfl_sync(FULL, x, base + i);
+            v = x * (1.0f / s);
+        }
+        if (on) w[e] = v;
     }
     __syncwarp();
 }
