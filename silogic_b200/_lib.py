@@ -130,12 +130,17 @@ def declare(name, argtypes):
         fn.restype = ctypes.c_int
 
 
+_fns = {}       # name -> entry point, filled by call()
+
+
 def call(name, *args):
     """Invoke ``name`` and raise :class:`SilogicError` on a non-zero status."""
-    L = lib()
-    st = getattr(L, name)(*args)
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(lib(), name)
+    st = fn(*args)
     if st != 0:
-        msg = L.slg_last_error().decode(errors="replace")
+        msg = lib().slg_last_error().decode(errors="replace")
         raise SilogicError(f"{name} failed with status {st}: {msg}")
 
 
@@ -151,7 +156,8 @@ def stream_ptr(device=None):
 
 
 def ptr(t):
-    return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
+    """Device address of a tensor for a ``c_void_p`` argument (``None``: NULL)."""
+    return t.data_ptr() if t is not None else None
 
 
 def require_cuda(*tensors):

@@ -295,9 +295,9 @@ DTYPE_ID = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 def embed_fwd(ids: Tensor, weight: Tensor, scale: float) -> Tensor:
     """``scale * weight[ids]``: ids int32 / int64 of any shape, weight ``[V, D]``."""
     V, D = weight.shape
-    out = torch.empty(ids.shape + (D,), dtype=weight.dtype, device=weight.device)
-    call("slg_embed_fwd", ptr(ids), ids.dtype == torch.int64, ids.numel(), ptr(weight),
-         DTYPE_ID[weight.dtype], V, D, scale, ptr(out), stream_ptr(weight.device))
+    out = weight.new_empty(ids.shape + (D,))
+    call("slg_embed_fwd", ids.data_ptr(), ids.dtype is torch.int64, ids.numel(), weight.data_ptr(),
+         DTYPE_ID[weight.dtype], V, D, scale, out.data_ptr(), stream_ptr(weight.device))
     return out
 
 
@@ -312,11 +312,11 @@ def embed_bwd(ids: Tensor, g: Tensor, V: int, scale: float, padding_idx: int) ->
     g = g.contiguous()
     D = g.shape[-1]
     N, dt = ids.numel(), DTYPE_ID[g.dtype]
-    gw = torch.empty((V, D), dtype=g.dtype, device=g.device)
+    gw = g.new_empty((V, D))
     nbytes = lib().slg_embed_bwd_workspace_bytes(N, V, D, dt)
-    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=g.device)
-    call("slg_embed_bwd", ptr(ids), ids.dtype == torch.int64, N, ptr(g), dt, V, D, scale,
-         padding_idx, ptr(gw), ptr(ws), nbytes, stream_ptr(g.device))
+    ws = g.new_empty((nbytes + 16,), dtype=torch.uint8)
+    call("slg_embed_bwd", ids.data_ptr(), ids.dtype is torch.int64, N, g.data_ptr(), dt, V, D, scale,
+         padding_idx, gw.data_ptr(), ws.data_ptr(), nbytes, stream_ptr(g.device))
     return gw
 
 
@@ -334,13 +334,15 @@ def ckpt_store(x: Tensor) -> Tuple[Tensor, Tensor]:
     """``[rows, cols]`` (rows may be strided) -> (codes uint8 ``[rows, ldc]``, bounds fp32
     ``[rows, blocks, 2]``)."""
     require_cuda(x)
-    if x.stride(1) != 1 or x.stride(0) < x.shape[1]:
-        x = x.contiguous()
     rows, cols = x.shape
-    codes = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.uint8, device=x.device)
-    bounds = torch.empty((rows, -(-cols // CKPT_BLOCK), 2), dtype=torch.float32, device=x.device)
-    call("slg_ckpt_store", ptr(x), DTYPE_ID[x.dtype], rows, cols, max(x.stride(0), cols), ptr(codes),
-         codes.shape[1], ptr(bounds), stream_ptr(x.device))
+    ldx = x.stride(0)
+    if x.stride(1) != 1 or ldx < cols:
+        x = x.contiguous()
+        ldx = cols
+    codes = x.new_empty((rows, (cols + 15) // 16 * 16), dtype=torch.uint8)
+    bounds = x.new_empty((rows, -(-cols // CKPT_BLOCK), 2), dtype=torch.float32)
+    call("slg_ckpt_store", x.data_ptr(), DTYPE_ID[x.dtype], rows, cols, ldx, codes.data_ptr(),
+         codes.shape[1], bounds.data_ptr(), stream_ptr(x.device))
     return codes, bounds
 
 
@@ -356,8 +358,8 @@ def ckpt_load(codes: Tensor, bounds: Tensor, cols: int, dtype: torch.dtype) -> T
     """The ``[rows, cols]`` values that the codes stand for."""
     require_cuda(codes, bounds)
     rows = codes.shape[0]
-    x = torch.empty((rows, cols), dtype=dtype, device=codes.device)
-    call("slg_ckpt_load", ptr(codes), codes.shape[1], ptr(bounds), rows, cols, ptr(x),
+    x = bounds.new_empty((rows, cols), dtype=dtype)
+    call("slg_ckpt_load", codes.data_ptr(), codes.shape[1], bounds.data_ptr(), rows, cols, x.data_ptr(),
          DTYPE_ID[dtype], cols, stream_ptr(codes.device))
     return x
 

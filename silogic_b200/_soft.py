@@ -32,7 +32,8 @@ def _keep_checkpoint(ctx):
 
 def _store(xt, meta):
     """Codes and bounds of the samples' columns (padding columns must not widen a block)."""
-    return op("ckpt_store")(xt[:, :meta.get("batch") or xt.shape[1]])
+    B = meta.get("batch")
+    return op("ckpt_store")(xt if B is None or B == xt.shape[1] else xt[:, :B])
 
 
 # ------------------------------------------------------------- transposes
@@ -152,11 +153,32 @@ def fc_layer_fm(layer, xt, wire_r=0, batch=None):
     return FCSoft.apply(xt, params, conn, meta)
 
 
+class FCSoftRows(torch.autograd.Function):
+    """:class:`FCSoft` between its two transposes, x [B, in] -> y [B, out]: one autograd node
+    for a layer that is called by itself (three cost its small calls more than the kernels)."""
+
+    @staticmethod
+    def forward(ctx, x, params, conn, meta):
+        ctx.shape = x.shape
+        B = x.shape[0]
+        xt = op("to_feature_major")(x.reshape(B, -1), ldb_for(B))
+        return op("from_feature_major")(FCSoft.forward(ctx, xt, params, conn, meta), B)
+
+    @staticmethod
+    def backward(ctx, gy):
+        B = ctx.shape[0]
+        gx, gparams, gconn, _ = FCSoft.backward(ctx, op("to_feature_major")(gy, ldb_for(B)))
+        if gx is not None:
+            gx = op("from_feature_major")(gx, B).view(ctx.shape)
+        return gx, gparams, gconn, None
+
+
 def logic_layer_forward(layer, x):
     """``LogicLayer.forward`` on ``[B, in]``."""
     require_cuda(x)
-    B = x.shape[0]
-    return FromFeatureMajor.apply(fc_layer_fm(layer, ToFeatureMajor.apply(x), batch=B), B)
+    meta, params, conn = _fc_meta(layer)
+    meta["batch"] = x.shape[0]
+    return FCSoftRows.apply(x, params, conn, meta)
 
 
 def node_forward(node, x, idx):

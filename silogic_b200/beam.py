@@ -34,7 +34,7 @@ def beam_step(logits, scores, finished=None, eos=None, width=None):
     V = logits.shape[-1] if logits.dim() else 0
     if V >= 1 << 27:
         raise ValueError(f"beam_step: vocabulary of {V} (must be below 2**27)")
-    if tuple(logits.shape) not in ((B, beams, V), (B * beams, V)):
+    if logits.shape != (B * beams, V) and logits.shape != (B, beams, V):
         raise ValueError(f"beam_step: logits {tuple(logits.shape)} do not fit scores {tuple(scores.shape)}")
     require_cuda(logits, scores, finished)
     width = beams if width is None else int(width)
@@ -51,14 +51,14 @@ def beam_step(logits, scores, finished=None, eos=None, width=None):
             raise ValueError("beam_step: finished must be bool, of the shape of scores")
         finished = finished.contiguous()
     dev = logits.device
-    x = logits.reshape(B * beams, V)
+    x = logits if logits.dim() == 2 else logits.reshape(B * beams, V)
     if B and (x.stride(1) != 1 and V > 1 or x.stride(0) < V):
         x = x.contiguous()
     scores = scores.float().contiguous()
-    out = torch.empty((B, width), dtype=torch.float32, device=dev)
-    parents = torch.empty((B, width), dtype=torch.int64, device=dev)
-    tokens = torch.empty((B, width), dtype=torch.int64, device=dev)
-    done = torch.empty((B, width), dtype=torch.bool, device=dev) if eos is not None else None
+    out = scores.new_empty((B, width))
+    parents = scores.new_empty((B, width), dtype=torch.int64)
+    tokens = torch.empty_like(parents)
+    done = scores.new_empty((B, width), dtype=torch.bool) if eos is not None else None
     call("slg_beam_step", x.data_ptr(), DTYPE_ID[x.dtype], B, beams, V, max(x.stride(0), V), scores.data_ptr(),
          ptr(finished), -1 if eos is None else int(eos), width, out.data_ptr(), parents.data_ptr(),
          tokens.data_ptr(), ptr(done), stream_ptr(dev))
@@ -86,8 +86,8 @@ def beam_reorder(state, parents, layout="rows", beams=None):
             beams = state.shape[0] // B if B else width
         if state.dim() < 1 or state.shape[0] != B * beams:
             raise ValueError(f"beam_reorder: {tuple(state.shape)} does not hold {B} entries of {beams} beams")
-        out = torch.empty((B * width,) + tuple(state.shape[1:]), dtype=state.dtype, device=state.device)
-        nbytes = out[0].numel() * out.element_size() if B else 0
+        out = state.new_empty((B * width,) + tuple(state.shape[1:]))
+        nbytes = out.numel() * out.element_size() // (B * width) if B else 0
         call("slg_beam_reorder_rows", ptr(state), nbytes, ptr(parents), B, beams, width, ptr(out), st)
         return out
     beams = width if beams is None else int(beams)
@@ -102,6 +102,6 @@ def beam_reorder(state, parents, layout="rows", beams=None):
     F, ld = state.shape
     if beams < 1 or ld * size < B * beams:
         raise ValueError(f"beam_reorder: rows of {ld} do not hold {B} entries of {beams} beams")
-    out = torch.empty((F, ld if beams == width else ld_for(B * width)), dtype=want, device=state.device)
+    out = torch.empty_like(state) if beams == width else state.new_empty((F, ld_for(B * width)))
     call(fn, ptr(state), F, ld, ptr(parents), B, beams, width, ptr(out), out.shape[1], st)
     return out

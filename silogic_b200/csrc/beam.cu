@@ -26,6 +26,30 @@ constexpr float BM_LARGEST = 3.402823466e+38f;
 // NaN -> -inf, +inf -> the largest finite value (fmaxf returns its other argument for NaN)
 __device__ __forceinline__ float clean(float v) { return fminf(fmaxf(v, -CUDART_INF_F), BM_LARGEST); }
 
+__device__ __forceinline__ float max_nan(float a, float b) {     // NaN when either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+constexpr float BM_LOG2E = 1.4426950408889634f;
+__device__ __forceinline__ float exp2_fast(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float exp_fast(float v) { return exp2_fast(v * BM_LOG2E); }
+
+// A lane's sum of exp(x - m) runs as s = sum 2^(x log2(e) - ref) with ref = m log2(e) rounded to
+// 32 bits: a term is one multiply-add (one rounding, like x - m), one exponential and one
+// addition.  ref's own rounding is a factor common to the terms, divided out at the end.  It
+// grows with m: from |m| = 65,536 on (masks at a type's lowest value) terms are
+// exp(x - m) as written.
+__device__ __forceinline__ bool large(float m) { return fabsf(m) >= 65536.0f; }
+__device__ __forceinline__ float rounding_of(float m) {     // log2 of the factor in s
+    return large(m) ? 0.0f : fmaf(m, BM_LOG2E, -(m * BM_LOG2E));
+}
+
 // Candidate order as one integer: larger value first, then the lower index.  0 = none.
 __device__ __forceinline__ uint32_t ordered(float v) {
     const uint32_t u = __float_as_uint(v + 0.0f);           // -0 -> +0
@@ -90,14 +114,12 @@ __device__ __forceinline__ void load_logits(const T* __restrict__ row, bool alig
     constexpr int E = Pack16<T>::E;
     if (aligned && at + E <= V) {
         unpack16<T>(__ldg(reinterpret_cast<const uint4*>(row + at)), x);
-#pragma unroll
-        for (int j = 0; j < E; ++j) x[j] = clean(x[j]);
         valid |= ((1u << E) - 1u) << bit;
     } else {
 #pragma unroll
         for (int j = 0; j < E; ++j) {
             const bool on = at + j < V;
-            x[j] = on ? clean(to_f32(row[at + j])) : -CUDART_INF_F;
+            x[j] = on ? to_f32(row[at + j]) : -CUDART_INF_F;
             valid |= (on ? 1u : 0u) << (bit + j);
         }
     }
@@ -148,14 +170,29 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
                     load_logits<T>(row, aligned, base + j * 32 * E, V, x + j * E, valid, j * E);
                 float top = x[0];
 #pragma unroll
-                for (int i = 1; i < BM_PER; ++i) top = fmaxf(top, x[i]);
+                for (int i = 1; i < BM_PER; ++i) top = max_nan(top, x[i]);
+                if (!(top < CUDART_INF_F)) {                // a NaN or +inf among them
+#pragma unroll
+                    for (int i = 0; i < BM_PER; ++i) x[i] = clean(x[i]);
+                    top = x[0];
+#pragma unroll
+                    for (int i = 1; i < BM_PER; ++i) top = fmaxf(top, x[i]);
+                }
                 if (top > m) {
-                    s *= __expf(m - top);                           // exp(-inf) = 0 at the start
+                    s *= exp2_fast(rounding_of(top) - rounding_of(m)) * exp_fast(m - top);     // s = 0 at the start
                     m = top;
                 }
-                const float ref = m > -CUDART_INF_F ? m : 0.0f;
+                if (!__any_sync(0xffffffffu, large(m))) {
+                    const float ref = m * BM_LOG2E;
 #pragma unroll
-                for (int i = 0; i < BM_PER; ++i) s += __expf(x[i] - ref);
+                    for (int i = 0; i < BM_PER; ++i) s += exp2_fast(fmaf(x[i], BM_LOG2E, -ref));
+                } else {                                    // also while all logits are masked
+                    const float ref = m > -CUDART_INF_F ? m : 0.0f, factor = exp2_fast(rounding_of(m));
+                    float t = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < BM_PER; ++i) t += exp_fast(x[i] - ref);
+                    s = fmaf(t, factor, s);
+                }
                 // Logits that can enter the list beat its last entry; while it is being filled,
                 // also the `width`-th largest of the lanes' maxima (so many logits reach that).
                 uint64_t bar = __shfl_sync(0xffffffffu, list, width - 1);
@@ -198,7 +235,7 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
         float mw = m;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) mw = fmaxf(mw, __shfl_xor_sync(0xffffffffu, mw, o));
-        float sw = m > -CUDART_INF_F ? s * __expf(m - mw) : 0.0f;
+        float sw = m > -CUDART_INF_F ? s * exp2_fast(-rounding_of(m)) * exp_fast(m - mw) : 0.0f;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sw += __shfl_xor_sync(0xffffffffu, sw, o);
         if (!waited) {
@@ -223,7 +260,7 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         float s = 0.0f;
         for (int i = b * parts + lane; i < (b + 1) * parts; i += 32)
-            if (own.m[i] > -CUDART_INF_F) s += own.s[i] * expf(own.m[i] - m);
+            if (own.m[i] > -CUDART_INF_F) s += own.s[i] * exp_fast(own.m[i] - m);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (lane == 0) { beam_m[b] = m; beam_l[b] = logf(s); }
@@ -325,11 +362,13 @@ reorder_features_kernel(const float* __restrict__ in, int64_t F, int64_t ldi, in
 
 // The same on bits.  A thread builds one 32-bit word of a row bit by bit; a CTA's threads
 // walk (row, word) of 32 word columns, row by row, so stores are whole lines (a warp that
-// built one word by ballot stored 4 bytes at a time: 10 us instead of 4 on 10,000 x 512).
-// The sources of the 1,024 samples are worked out once per CTA.
+// built one word by ballot stored 4 bytes at a time: 10 us on 10,000 x 512).  The sources of the
+// 1,024 samples are worked out once per CTA.  With width >= beams a word's sources lie in
+// four words, which are loaded first.
 constexpr int RP_THREADS = 256;
 constexpr int RP_WORDS = 32;
 constexpr int RP_PER = 2;               // words per thread
+template <bool FOUR>
 __global__ void __launch_bounds__(RP_THREADS)
 reorder_packed_kernel(const uint32_t* __restrict__ in, int64_t F, int64_t ldi, int64_t n,
                       const int64_t* __restrict__ parents, int beams, int width, uint32_t* __restrict__ out,
@@ -339,10 +378,9 @@ reorder_packed_kernel(const uint32_t* __restrict__ in, int64_t F, int64_t ldi, i
     const int64_t w0 = (int64_t)blockIdx.y * RP_WORDS;
     const int words = (int)min((int64_t)RP_WORDS, ldo - w0);
     for (int i = threadIdx.x; i < words * 32; i += RP_THREADS) {
-        // an output word's 32 samples span at most 32 / width + 2 entries of at most 32
-        // beams: their sources lie within 32 * 34 samples after the first entry's
+        // an output word's 32 samples span at most 31 / width + 2 entries of at most 32 beams
         const int64_t r0 = (w0 + i / 32) * 32, r = r0 + i % 32;
-        const int64_t first = (r0 / width * beams) >> 5;
+        const int64_t first = ((int64_t)((uint32_t)r0 / (uint32_t)width) * beams) >> 5;
         from[i / 32][i % 32] =
             r < n ? (uint16_t)(beam_source(parents, (uint32_t)r, beams, width) - first * 32) : (uint16_t)0xffff;
         if (i % 32 == 0) word_of[i / 32] = first;
@@ -355,12 +393,28 @@ reorder_packed_kernel(const uint32_t* __restrict__ in, int64_t F, int64_t ldi, i
         if (t >= total) continue;
         const int64_t f = total < (1ll << 32) ? (int64_t)((uint32_t)t / (uint32_t)words) : t / words;
         const int w = (int)(t - f * words);
-        const uint32_t* src = in + f * ldi + word_of[w];
+        const int64_t first = word_of[w];
+        const uint32_t* src = in + f * ldi + first;
         uint32_t bits = 0;
+        if constexpr (FOUR) {
+            // the word's first sample is at most width - 1 into its entry, so its last one's
+            // entry begins at most (width + 30) beams / width <= 62 samples after the first's:
+            // offsets stay below 31 + 62 + 32 < 128
+            uint32_t x[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x[q] = first + q < ldi ? __ldg(src + q) : 0u;
 #pragma unroll 8
-        for (int j = 0; j < 32; ++j) {
-            const uint32_t s = from[w][j];
-            if (s != 0xffffu) bits |= (__ldg(src + (s >> 5)) >> (s & 31u) & 1u) << j;
+            for (int j = 0; j < 32; ++j) {
+                const uint32_t s = from[w][j];
+                const uint32_t lo = s & 32u ? x[1] : x[0], hi = s & 32u ? x[3] : x[2];
+                if (s != 0xffffu) bits |= ((s & 64u ? hi : lo) >> (s & 31u) & 1u) << j;
+            }
+        } else {
+#pragma unroll 8
+            for (int j = 0; j < 32; ++j) {
+                const uint32_t s = from[w][j];
+                if (s != 0xffffu) bits |= (__ldg(src + (s >> 5)) >> (s & 31u) & 1u) << j;
+            }
         }
         out[f * ldo + w0 + w] = bits;
     }
@@ -449,8 +503,11 @@ extern "C" int slg_beam_reorder_packed(const uint64_t* in, int64_t F, int64_t ld
     const int64_t per_row = std::min<int64_t>(2 * ldo, RP_WORDS), tiles = cdiv(2 * ldo, RP_WORDS);
     if (tiles > 65535) return set_error(SLG_ERR_ARG, "slg_beam_reorder_packed: batch too large");
     const dim3 grid((unsigned)cdiv(F * per_row, RP_THREADS * RP_PER), (unsigned)tiles);
-    reorder_packed_kernel<<<grid, RP_THREADS, 0, as_stream(stream)>>>(reinterpret_cast<const uint32_t*>(in), F, 2 * ldi,
-                                                                     B * width, parents, beams, width,
-                                                                     reinterpret_cast<uint32_t*>(out), 2 * ldo);
+    auto go = [&](auto kernel) {
+        kernel<<<grid, RP_THREADS, 0, as_stream(stream)>>>(reinterpret_cast<const uint32_t*>(in), F, 2 * ldi, B * width,
+                                                           parents, beams, width, reinterpret_cast<uint32_t*>(out), 2 * ldo);
+    };
+    if (width >= beams) go(reorder_packed_kernel<true>);
+    else go(reorder_packed_kernel<false>);
     return check_launch("slg_beam_reorder_packed");
 }

@@ -61,54 +61,71 @@ __device__ __forceinline__ void block_of(int64_t q, int64_t nblk, int64_t& row, 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(CK_WARPS * 32)
+__global__ void __launch_bounds__(CK_WARPS * 32, 6)
 ckpt_store_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t ldx, int vec,
                   uint32_t* __restrict__ codes, int64_t ldw, float2* __restrict__ bounds, int64_t nblk) {
     const int lane = threadIdx.x & 31;
     const int64_t q0 = ((int64_t)blockIdx.x * CK_WARPS + (threadIdx.x >> 5)) * CK_UNIT;
     const int64_t total = rows * nblk;
     if (q0 >= total) return;
-    int64_t row, blk;
-    block_of(q0, nblk, row, blk);
+    int64_t row0, blk0;
+    block_of(q0, nblk, row0, blk0);
+    // row and columns of block u, worked out again where they are used: kept, they cost
+    // registers, and warps in flight are what this kernel lives on
+    auto place = [&](int u, int64_t& row, int64_t& c) {
+        row = row0;
+        int64_t blk = blk0 + u;
+        while (blk >= nblk) { blk -= nblk; ++row; }
+        c = blk * CK_BLOCK + lane * 4;
+        const int64_t left = cols - c;
+        return q0 + u >= total || left <= 0 ? 0 : left < 4 ? (int)left : 4;     // the lane's values
+    };
     float v[CK_UNIT][4];
-    int64_t word_at[CK_UNIT];       // the lane's code word, -1: none
-    int n[CK_UNIT];                 // its values
+    int counts = 0;
 #pragma unroll
     for (int u = 0; u < CK_UNIT; ++u) {
-        const int64_t c = blk * CK_BLOCK + lane * 4;
-        const bool on = q0 + u < total && c < cols;
-        n[u] = on ? (int)(cols - c < 4 ? cols - c : 4) : 0;
-        word_at[u] = row * ldw + (c >> 2);
-        if (on) load4(x + row * ldx, c, cols, vec, v[u]);
-        if (++blk == nblk) { blk = 0; ++row; }
+        int64_t row, c;
+        const int n = place(u, row, c);
+        counts |= n << (4 * u);
+        if (n) load4(x + row * ldx, c, cols, vec, v[u]);
     }
-    float2 mine = make_float2(0.f, 0.f);
+    float lo[CK_UNIT], my_lo = 0.0f, my_range = 0.0f;
 #pragma unroll
     for (int u = 0; u < CK_UNIT; ++u) {
-        float lo = CUDART_INF_F, hi = -CUDART_INF_F;
+        float l = CUDART_INF_F, h = -CUDART_INF_F;
+        const int n = counts >> (4 * u) & 7;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (j < n[u]) {
-                lo = fminf(lo, v[u][j]);
-                hi = max_nan_f32(hi, v[u][j]);
+            if (j < n) {
+                l = fminf(l, v[u][j]);
+                h = max_nan_f32(h, v[u][j]);
             }
-        lo = warp_min_f32(lo);
-        hi = warp_max_nan_f32(hi);
-        const float range = __fsub_rn(hi, lo);              // NaN or infinite: something is not finite
-        const bool bad = !isfinite(range);
-        const float step = __fmul_rn(range, 1.0f / 255.0f);
-        const bool flat = bad || step < CK_TINY;
-        const float inv = flat ? 0.0f : __fdiv_rn(255.0f, range);
-        uint32_t word = 0;
+        lo[u] = warp_min_f32(l);
+        const float range = __fsub_rn(warp_max_nan_f32(h), lo[u]);      // NaN or infinite: something is not finite
+        if (lane == u) { my_lo = lo[u]; my_range = range; }
+    }
+    // lane u works out block u's step and its inverse: one division per warp
+    const bool bad = !isfinite(my_range);
+    const float step = __fmul_rn(my_range, 1.0f / 255.0f);
+    const bool flat = bad || step < CK_TINY;
+    const float my_inv = flat ? 0.0f : __fdiv_rn(255.0f, my_range);
+    const float2 mine = bad ? make_float2(CUDART_NAN_F, CUDART_NAN_F) : make_float2(my_lo, flat ? 0.0f : step);
+#pragma unroll
+    for (int u = 0; u < CK_UNIT; ++u) {
+        const float inv = __shfl_sync(0xffffffffu, my_inv, u);
+        // Adding 1.5 2^23 rounds to the nearest even integer, as rint does, and leaves it in the
+        // low byte (0 <= code <= 255 as lo <= x <= hi); conversion instructions run at an
+        // eighth of the rate.
+        uint32_t bits[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (!flat && j < n[u]) {
-                const float code = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(v[u][j], lo), inv)), 0.0f), 255.0f);
-                word |= (uint32_t)code << (8 * j);
-            }
-        if (n[u]) codes[word_at[u]] = word;
-        if (lane == u)
-            mine = bad ? make_float2(CUDART_NAN_F, CUDART_NAN_F) : make_float2(lo, flat ? 0.0f : step);
+            bits[j] = __float_as_uint(__fadd_rn(__fmul_rn(__fsub_rn(v[u][j], lo[u]), inv), 12582912.0f));
+        uint32_t word = __byte_perm(__byte_perm(bits[0], bits[1], 0x0040), __byte_perm(bits[2], bits[3], 0x0040), 0x5410);
+        if (inv == 0.0f) word = 0;                          // a constant block, or one that is not finite
+        int64_t row, c;
+        const int n = place(u, row, c);
+        if (n < 4) word &= (1u << (8 * n)) - 1u;
+        if (n) codes[row * ldw + (c >> 2)] = word;
     }
     if (lane < CK_UNIT && q0 + lane < total) bounds[q0 + lane] = mine;
 }

@@ -93,7 +93,7 @@ struct KeysOfPairs {
     __device__ __forceinline__ uint32_t pos(int64_t i) const { return p[i]; }
 };
 
-constexpr int RK_MAX = 8192;
+constexpr int RK_MAX = 8192;            // 13 us; the radix sort's four launches take 26 up to 16,384
 constexpr int RK_THREADS = 256;
 constexpr int RK_WARPS = RK_THREADS / 32;
 
@@ -347,6 +347,7 @@ __device__ __forceinline__ void store_carry(float* __restrict__ p, int lane, con
 
 constexpr int SG_WARPS = 4;
 constexpr int SG_UNROLL = 8;
+constexpr int SG_CHUNK = 128;       // largest chunk
 
 // head_row[chunk] = row that ends in this chunk but began earlier, else -1;
 // start[row] = chunk with the row's first entry, for rows that end in a later one
@@ -358,6 +359,7 @@ embed_sum_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ 
     constexpr int E = Pack16<T>::E;
     constexpr int SLICE = 32 * E;
     __shared__ Cut cut[2];
+    __shared__ uint32_t skey[SG_CHUNK], spos[SG_CHUNK];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t total = V + N;
     const int64_t c = blockIdx.x;
@@ -368,15 +370,20 @@ embed_sum_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ 
     }
     __syncthreads();
     const int64_t r0 = cut[0].r, i0 = cut[0].i, r1 = cut[1].r;
-    int64_t i1 = cut[1].i;
+    int n = (int)(cut[1].i - i0);                       // the chunk's entries: at most SG_CHUNK
+    for (int i = threadIdx.x; i < n; i += SG_WARPS * 32) {
+        skey[i] = key[i0 + i];
+        spos[i] = pos[i0 + i];
+    }
     const bool begun = r0 < V && i0 > 0 && (int64_t)key[i0 - 1] == r0;      // r0 has entries in earlier chunks
-    const bool open = r1 < V && i1 > i0 && (int64_t)key[i1 - 1] == r1;      // r1 goes on in the next one
+    __syncthreads();
+    const bool open = r1 < V && n > 0 && (int64_t)skey[n - 1] == r1;        // r1 goes on in the next one
     if (threadIdx.x == 0 && blockIdx.y == 0) {
         head_row[c] = begun && r1 > r0 ? (int32_t)r0 : -1;
         if (open && !(begun && r1 == r0)) start[r1] = (int32_t)c;
     }
     if (r1 == V) {                      // what follows the last row's end has no gradient
-        while (i1 > i0 && (int64_t)key[i1 - 1] >= V) --i1;
+        while (n > 0 && (int64_t)skey[n - 1] >= V) --n;
     }
     for (int64_t s = (int64_t)blockIdx.y * SG_WARPS + warp; s < slices; s += (int64_t)gridDim.y * SG_WARPS) {
         const int64_t c0 = s * SLICE;
@@ -394,18 +401,15 @@ embed_sum_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ 
                 for (int j = 0; j < E; ++j) acc[j] = 0.0f;
             }
         };
-        for (int64_t i = i0; i < i1; i += SG_UNROLL) {
+        for (int i = 0; i < n; i += SG_UNROLL) {
             Cols<T, VEC> v[SG_UNROLL];
-            uint32_t k[SG_UNROLL];
+#pragma unroll
+            for (int u = 0; u < SG_UNROLL; ++u)
+                if (i + u < n) v[u].load(g + (int64_t)spos[i + u] * D, c0, D, lane);
 #pragma unroll
             for (int u = 0; u < SG_UNROLL; ++u) {
-                k[u] = i + u < i1 ? key[i + u] : 0u;
-                if (i + u < i1) v[u].load(g + (int64_t)pos[i + u] * D, c0, D, lane);
-            }
-#pragma unroll
-            for (int u = 0; u < SG_UNROLL; ++u) {
-                if (i + u >= i1) break;
-                end_rows((int64_t)k[u]);
+                if (i + u >= n) break;
+                end_rows((int64_t)skey[i + u]);
                 v[u].add_to(acc);
             }
         }
@@ -503,7 +507,7 @@ static EmbedPlan embed_plan(int64_t N, int64_t V, int64_t D, int es) {
     p.slices = cdiv(D * es, 512);                           // 32 lanes x 16 bytes
     // about 16 chunks per SM, between 16 items (a chunk costs two searches) and 128
     p.chunk = 16;
-    while (p.chunk < 128 && (V + N) / p.chunk > 148 * 16) p.chunk *= 2;
+    while (p.chunk < SG_CHUNK && (V + N) / p.chunk > 148 * 16) p.chunk *= 2;
     p.nchunk = cdiv(V + N, p.chunk);
     p.hist_at = up(4 * 4 * N);                              // two (token, position) buffers
     p.head_at = p.hist_at + up(p.tiles * RS_BINS * 4);

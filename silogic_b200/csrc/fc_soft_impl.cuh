@@ -14,6 +14,8 @@
 // the finish kernel that sums the chunks and applies the softmax Jacobians is
 // deterministic.
 #pragma once
+#include <type_traits>
+
 #include "soft_common.cuh"
 
 namespace slg {
@@ -79,30 +81,40 @@ fc_soft_fwd_kernel(const float4* __restrict__ x, int64_t nv, const int32_t* __re
             rows[j * KT + k] = x + (on ? (int64_t)S.cand[j * K + k] * nv : 0);
             wr[j * KT + k] = on ? S.w[j * K + k] : 0.0f;
         }
-    for (int it = 0; it < FS_ITER; ++it) {
-        const int64_t v = v0 + it * 32 + lane;
-        if (v >= nv) break;
-        float a[4][AR];
+    // Zero weights (one-hot selection) skip their loads; a node that has none takes the loop
+    // without the tests, which cost a tenth of the time (10,000 Top-8 Walsh nodes x 4,096
+    // samples: 285 -> 226 us).
+    bool dense = true;
 #pragma unroll
-        for (int j = 0; j < AR; ++j) {
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int e = 0; e < AR * KT; ++e) dense = dense && (e % KT >= K || wr[e] != 0.0f);
+    auto walk = [&](auto skip_zeros) {
+        for (int it = 0; it < FS_ITER; ++it) {
+            const int64_t v = v0 + it * 32 + lane;
+            if (v >= nv) break;
+            float a[4][AR];
 #pragma unroll
-            for (int k = 0; k < KT; ++k) {
-                if (k < K && wr[j * KT + k] != 0.0f) {     // skip one-hot zeros
-                    const float wk = wr[j * KT + k];
-                    const float4 xv = __ldg(rows[j * KT + k] + v);
-                    acc.x += wk * xv.x; acc.y += wk * xv.y; acc.z += wk * xv.z; acc.w += wk * xv.w;
+            for (int j = 0; j < AR; ++j) {
+                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int k = 0; k < KT; ++k) {
+                    if (k < K && (!decltype(skip_zeros)::value || wr[j * KT + k] != 0.0f)) {
+                        const float wk = wr[j * KT + k];
+                        const float4 xv = __ldg(rows[j * KT + k] + v);
+                        acc.x += wk * xv.x; acc.y += wk * xv.y; acc.z += wk * xv.z; acc.w += wk * xv.w;
+                    }
                 }
+                a[0][j] = acc.x; a[1][j] = acc.y; a[2][j] = acc.z; a[3][j] = acc.w;
             }
-            a[0][j] = acc.x; a[1][j] = acc.y; a[2][j] = acc.z; a[3][j] = acc.w;
+            float4 r;
+            r.x = node_fwd<NODE, AR>(S.np, a[0]);
+            r.y = node_fwd<NODE, AR>(S.np, a[1]);
+            r.z = node_fwd<NODE, AR>(S.np, a[2]);
+            r.w = node_fwd<NODE, AR>(S.np, a[3]);
+            y[o * nv + v] = r;
         }
-        float4 r;
-        r.x = node_fwd<NODE, AR>(S.np, a[0]);
-        r.y = node_fwd<NODE, AR>(S.np, a[1]);
-        r.z = node_fwd<NODE, AR>(S.np, a[2]);
-        r.w = node_fwd<NODE, AR>(S.np, a[3]);
-        y[o * nv + v] = r;
-    }
+    };
+    if (dense) walk(std::false_type{});
+    else walk(std::true_type{});
 }
 
 // partials layout: ws[chunk][o][NPART], NPART = AR*K + NPG (conn grads first)

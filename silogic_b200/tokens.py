@@ -12,7 +12,7 @@ class _TokenEmbedding(torch.autograd.Function):
     def forward(ctx, ids, weight, scale, padding_idx):
         ctx.save_for_backward(ids)
         ctx.args = (weight.shape[0], scale, padding_idx)
-        return op("embed_fwd")(ids, weight, scale)
+        return op("embed_fwd")(ids, weight.contiguous(), scale)
 
     @staticmethod
     def backward(ctx, g):
@@ -31,27 +31,26 @@ def token_embedding(ids, weight, scale=1.0, padding_idx=None, check=False):
     if weight.dim() != 2 or weight.dtype not in DTYPE_ID:
         raise TypeError("token_embedding: weight must be [V, D] float32, bfloat16 or float16, got "
                         f"{tuple(weight.shape)} {weight.dtype}")
-    if ids.dtype != torch.int64 and ids.dtype != torch.int32:
+    if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
         raise TypeError(f"token_embedding: ids must be int32 or int64, got {ids.dtype}")
-    require_cuda(ids, weight)
+    if not (ids.is_cuda and weight.is_cuda):
+        require_cuda(ids, weight)
     if ids.device != weight.device:
         raise ValueError(f"token_embedding: ids on {ids.device}, weight on {weight.device}")
-    V = weight.shape[0]
-    if V == 0 or weight.shape[1] == 0:
+    V, D = weight.shape
+    if V == 0 or D == 0:
         raise ValueError(f"token_embedding: empty weight {tuple(weight.shape)}")
-    if padding_idx is None:
-        pad = -1
-    else:
-        pad = int(padding_idx)
-        if not -V <= pad < V:
+    pad = -1
+    if padding_idx is not None:
+        if not -V <= padding_idx < V:
             raise ValueError(f"token_embedding: padding_idx {padding_idx} not in [-{V}, {V})")
-        pad %= V
+        pad = int(padding_idx) % V
     if check:
         _hard.check_index_range(ids, V, "token ids")
-    ids, weight = ids.contiguous(), weight.contiguous()
-    if torch.is_grad_enabled() and weight.requires_grad:
+    ids = ids.contiguous()
+    if weight.requires_grad and torch.is_grad_enabled():
         return _TokenEmbedding.apply(ids, weight, float(scale), pad)
-    return op("embed_fwd")(ids, weight, float(scale))
+    return op("embed_fwd")(ids, weight.contiguous(), float(scale))
 
 
 class TokenEmbedding(nn.Module):
