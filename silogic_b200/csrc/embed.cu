@@ -101,11 +101,12 @@ constexpr int RK_WARPS = RK_THREADS / 32;
 // at earlier positions count when they are <= its own, later ones when they are <.
 template <typename I>
 __global__ void __launch_bounds__(RK_THREADS)
-rank_sort_kernel(KeysOfIds<I> src, int N, uint32_t* __restrict__ ko, uint32_t* __restrict__ po) {
+rank_sort_kernel(KeysOfIds<I> src, int N, uint32_t* __restrict__ ko, uint32_t* __restrict__ po, int32_t* __restrict__ zero) {
     __shared__ alignas(16) uint32_t key[RK_MAX];
     __shared__ int part[RK_WARPS][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n4 = (N + 3) & ~3;
+    if (blockIdx.x == 0 && threadIdx.x < 2) zero[threadIdx.x] = 0;
     for (int i = threadIdx.x; i < n4; i += RK_THREADS) key[i] = i < N ? src.key(i) : 0xffffffffu;
     __syncthreads();
     const int i0 = blockIdx.x * 32, i = i0 + lane;
@@ -152,8 +153,10 @@ __host__ __device__ inline int64_t rs_span(int64_t N) {   // keys per CTA: whole
 // hist[cta][digit]
 template <typename S>
 __global__ void __launch_bounds__(RS_THREADS)
-radix_count_kernel(S src, int64_t N, int64_t span, int shift, uint32_t mask, uint32_t* __restrict__ hist) {
+radix_count_kernel(S src, int64_t N, int64_t span, int shift, uint32_t mask, uint32_t* __restrict__ hist,
+                   int32_t* __restrict__ zero) {
     __shared__ uint32_t h[RS_BINS];
+    if (blockIdx.x == 0 && threadIdx.x < 2) zero[threadIdx.x] = 0;
     h[threadIdx.x] = 0;
     __syncthreads();
     const int64_t a = (int64_t)blockIdx.x * span, b = a + span < N ? a + span : N;
@@ -188,11 +191,15 @@ radix_scatter_kernel(S src, int64_t N, int64_t span, int shift, int bits, const 
     };
     load(a + warp * (32 * RS_PER) + lane);
     uint32_t before = 0, all = 0;
-#pragma unroll 16
-    for (int t = 0; t < (int)gridDim.x; ++t) {
-        const uint32_t c = hist[(int64_t)t * RS_BINS + d];
-        before += t < (int)blockIdx.x ? c : 0u;
-        all += c;
+    for (int t0 = 0; t0 < (int)gridDim.x; t0 += 32) {      // 32 loads at a time: this is latency
+        uint32_t c[32];
+#pragma unroll
+        for (int q = 0; q < 32; ++q) c[q] = t0 + q < (int)gridDim.x ? __ldg(&hist[(int64_t)(t0 + q) * RS_BINS + d]) : 0u;
+#pragma unroll
+        for (int q = 0; q < 32; ++q) {
+            before += t0 + q < (int)blockIdx.x ? c[q] : 0u;
+            all += c[q];
+        }
     }
     uint32_t inc = all;                                    // inclusive scan over digits
 #pragma unroll
@@ -348,14 +355,18 @@ __device__ __forceinline__ void store_carry(float* __restrict__ p, int lane, con
 constexpr int SG_WARPS = 4;
 constexpr int SG_UNROLL = 8;
 constexpr int SG_CHUNK = 128;       // largest chunk
+constexpr int JN_WARPS = 8;
+constexpr int JN_SHORT = 8;
 
-// head_row[chunk] = row that ends in this chunk but began earlier, else -1;
-// start[row] = chunk with the row's first entry, for rows that end in a later one
+// head_row[chunk] = row that ends in this chunk but began earlier; cuts: the lists of such
+// chunks, in any order -- every one is joined by itself -- those of long rows from the end
+// backwards, with their lengths in cut_count; start[row] = chunk with the row's first entry.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(SG_WARPS * 32)
 embed_sum_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ pos, int64_t N, int64_t V,
                  int64_t D, int64_t chunk, const T* __restrict__ g, float scale, T* __restrict__ gw,
-                 float* __restrict__ carry, int64_t slices, int32_t* __restrict__ head_row, int32_t* __restrict__ start) {
+                 float* __restrict__ carry, int64_t slices, int32_t* __restrict__ head_row, int32_t* __restrict__ start,
+                 int32_t* __restrict__ cuts, int32_t* __restrict__ cut_count) {
     constexpr int E = Pack16<T>::E;
     constexpr int SLICE = 32 * E;
     __shared__ Cut cut[2];
@@ -379,7 +390,14 @@ embed_sum_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ 
     __syncthreads();
     const bool open = r1 < V && n > 0 && (int64_t)skey[n - 1] == r1;        // r1 goes on in the next one
     if (threadIdx.x == 0 && blockIdx.y == 0) {
-        head_row[c] = begun && r1 > r0 ? (int32_t)r0 : -1;
+        if (begun && r1 > r0) {
+            head_row[c] = (int32_t)r0;
+            // long: the row also fills the JN_SHORT chunks before this one
+            const int64_t back = i0 - 1 - (JN_SHORT * chunk);
+            const bool lengthy = back >= 0 && (int64_t)key[back] == r0;
+            const int32_t at = atomicAdd(&cut_count[lengthy], 1);
+            cuts[lengthy ? gridDim.x - 1 - at : at] = (int32_t)c;
+        }
         if (open && !(begun && r1 == r0)) start[r1] = (int32_t)c;
     }
     if (r1 == V) {                      // what follows the last row's end has no gradient
@@ -418,38 +436,28 @@ embed_sum_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ 
     }
 }
 
-// One CTA = one cut row x a share of its groups of 128 columns.  Short rows: a warp per
-// group adds the row's tails, then its head.  Long ones (a frequent token's row is cut into
-// hundreds of chunks): the CTA's warps take equal runs of the tails, joined in shared memory.
-constexpr int JN_WARPS = 8;
-constexpr int JN_SHORT = 8;
-
+// Joins the cut rows, 128 columns at a time.  Short rows: a warp adds the row's tails, then
+// its head.  Long ones (a frequent token's row is cut into hundreds of chunks): a CTA's
+// warps take equal runs of the tails, joined in shared memory.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(JN_WARPS * 32)
 embed_join_kernel(int64_t D, float scale, T* __restrict__ gw, const float* __restrict__ carry, int64_t ldc,
-                  const int32_t* __restrict__ head_row, const int32_t* __restrict__ start) {
+                  const int32_t* __restrict__ head_row, const int32_t* __restrict__ start,
+                  const int32_t* __restrict__ cuts, const int32_t* __restrict__ cut_count, int64_t nchunk) {
     __shared__ float4 part[JN_WARPS][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t c = blockIdx.x;
-    const int64_t r = head_row[c];
-    if (r < 0) return;
-    const int64_t first = start[r], n = c - first;
+    const int64_t shorts = cut_count[0], longs = cut_count[1];
+    int64_t c = 0, r = 0, first = 0;
     const int64_t groups = ldc / 128;
     auto sum = [&](int64_t g, int64_t a, int64_t b) {           // tails of chunks first+a .. first+b-1
         const float4* p = reinterpret_cast<const float4*>(carry + (2 * (first + a) + 1) * ldc + g * 128) + lane;
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-        int64_t q = a;
-        for (; q + 8 <= b; q += 8) {
+        for (int64_t q = a; q < b; q += 8, p += 8 * (ldc / 2)) {
             float4 v[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = __ldg(p + (int64_t)u * (ldc / 2));
-            p += 8 * (ldc / 2);
+            for (int u = 0; u < 8; ++u) v[u] = q + u < b ? __ldg(p + (int64_t)u * (ldc / 2)) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int u = 0; u < 8; ++u) { s.x += v[u].x; s.y += v[u].y; s.z += v[u].z; s.w += v[u].w; }
-        }
-        for (; q < b; ++q, p += ldc / 2) {
-            const float4 v = __ldg(p);
-            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
         }
         return s;
     };
@@ -467,12 +475,15 @@ embed_join_kernel(int64_t D, float scale, T* __restrict__ gw, const float* __res
                 if (col + j < D) o[j] = from_f32<T>(v[j]);
         }
     };
-    if (n <= JN_SHORT) {
-        for (int64_t g = (int64_t)blockIdx.y * JN_WARPS + warp; g < groups; g += (int64_t)gridDim.y * JN_WARPS)
-            finish(g, sum(g, 0, n));
-        return;
-    }
-    for (int64_t g = blockIdx.y; g < groups; g += gridDim.y) {
+    auto pick = [&](int64_t at) {
+        c = cuts[at];
+        r = head_row[c];
+        first = start[r];
+    };
+    for (int64_t i = blockIdx.x; i < longs * groups; i += gridDim.x) {
+        const int64_t e = i / groups, g = i - e * groups;
+        pick(nchunk - 1 - e);
+        const int64_t n = c - first;
         part[warp][lane] = sum(g, n * warp / JN_WARPS, n * (warp + 1) / JN_WARPS);
         __syncthreads();
         if (warp == 0) {
@@ -486,11 +497,16 @@ embed_join_kernel(int64_t D, float scale, T* __restrict__ gw, const float* __res
         }
         __syncthreads();
     }
+    for (int64_t i = (int64_t)blockIdx.x * JN_WARPS + warp; i < shorts * groups; i += (int64_t)gridDim.x * JN_WARPS) {
+        const int64_t e = i / groups, g = i - e * groups;
+        pick(e);
+        finish(g, sum(g, 0, c - first));
+    }
 }
 
 // ------------------------------------------------------------------- plans
 struct EmbedPlan {
-    int64_t hist_at, head_at, start_at, carry_at, bytes;
+    int64_t hist_at, head_at, cuts_at, start_at, carry_at, bytes;
     int64_t chunk, nchunk, slices, tiles;
     int passes, bits;
 };
@@ -511,7 +527,8 @@ static EmbedPlan embed_plan(int64_t N, int64_t V, int64_t D, int es) {
     p.nchunk = cdiv(V + N, p.chunk);
     p.hist_at = up(4 * 4 * N);                              // two (token, position) buffers
     p.head_at = p.hist_at + up(p.tiles * RS_BINS * 4);
-    p.start_at = p.head_at + up(p.nchunk * 4);
+    p.cuts_at = p.head_at + up(p.nchunk * 4);               // lists of cut rows, then their two lengths
+    p.start_at = p.cuts_at + up(p.nchunk * 4 + 8);
     p.carry_at = p.start_at + up(V * 4);
     p.bytes = p.carry_at + p.nchunk * 2 * p.slices * (512 / es) * 4;
     return p;
@@ -545,10 +562,11 @@ static void embed_fwd_launch(const I* ids, int64_t N, const T* w, int64_t V, int
 template <typename I>
 static const uint32_t* embed_sort(const I* ids, int64_t N, int64_t V, int64_t pad, const EmbedPlan& p, char* ws,
                                   cudaStream_t st) {
+    int32_t* zero = reinterpret_cast<int32_t*>(ws + p.cuts_at) + p.nchunk;
     uint32_t* buf[2] = {reinterpret_cast<uint32_t*>(ws), reinterpret_cast<uint32_t*>(ws) + 2 * N};
     const KeysOfIds<I> in{ids, V, pad};
     if (N <= RK_MAX) {
-        rank_sort_kernel<I><<<(unsigned)cdiv(N, 32), RK_THREADS, 0, st>>>(in, (int)N, buf[0], buf[0] + N);
+        rank_sort_kernel<I><<<(unsigned)cdiv(N, 32), RK_THREADS, 0, st>>>(in, (int)N, buf[0], buf[0] + N, zero);
         return buf[0];
     }
     uint32_t* hist = reinterpret_cast<uint32_t*>(ws + p.hist_at);
@@ -559,11 +577,11 @@ static const uint32_t* embed_sort(const I* ids, int64_t N, int64_t V, int64_t pa
     for (int q = 0; q < p.passes; ++q) {
         uint32_t* dst = buf[q & 1];
         if (q == 0) {
-            radix_count_kernel<<<grid, RS_THREADS, 0, st>>>(in, N, span, 0, mask, hist);
+            radix_count_kernel<<<grid, RS_THREADS, 0, st>>>(in, N, span, 0, mask, hist, zero);
             radix_scatter_kernel<<<grid, RS_THREADS, 0, st>>>(in, N, span, 0, p.bits, hist, dst, dst + N);
         } else {
             const KeysOfPairs pairs{src, src + N};
-            radix_count_kernel<<<grid, RS_THREADS, 0, st>>>(pairs, N, span, p.bits * q, mask, hist);
+            radix_count_kernel<<<grid, RS_THREADS, 0, st>>>(pairs, N, span, p.bits * q, mask, hist, zero);
             radix_scatter_kernel<<<grid, RS_THREADS, 0, st>>>(pairs, N, span, p.bits * q, p.bits, hist, dst, dst + N);
         }
         src = dst;
@@ -578,15 +596,17 @@ static void embed_bwd_launch(const uint32_t* key, int64_t N, int64_t V, int64_t 
     float* carry = reinterpret_cast<float*>(ws + p.carry_at);
     int32_t* head = reinterpret_cast<int32_t*>(ws + p.head_at);
     int32_t* start = reinterpret_cast<int32_t*>(ws + p.start_at);
+    int32_t* cuts = reinterpret_cast<int32_t*>(ws + p.cuts_at);
+    int32_t* count = cuts + p.nchunk;
     const dim3 grid((unsigned)p.nchunk, (unsigned)std::min<int64_t>(cdiv(p.slices, SG_WARPS), 65535));
     const int64_t ldc = p.slices * 32 * E;
-    const dim3 jgrid((unsigned)p.nchunk, (unsigned)std::min<int64_t>(cdiv(ldc, 256), 4));
+    const unsigned jgrid = (unsigned)std::min<int64_t>(cdiv(p.nchunk * (ldc / 128), JN_WARPS), 4 * sm_count());
     auto go = [&](auto vec) {
         constexpr bool VEC = decltype(vec)::value;
         embed_sum_kernel<T, VEC><<<grid, SG_WARPS * 32, 0, st>>>(key, key + N, N, V, D, p.chunk, g, scale, gw, carry,
-                                                                 p.slices, head, start);
+                                                                 p.slices, head, start, cuts, count);
         if (N > 0)
-            embed_join_kernel<T, VEC><<<jgrid, JN_WARPS * 32, 0, st>>>(D, scale, gw, carry, ldc, head, start);
+            embed_join_kernel<T, VEC><<<jgrid, JN_WARPS * 32, 0, st>>>(D, scale, gw, carry, ldc, head, start, cuts, count, p.nchunk);
     };
     if (D % E == 0 && aligned16(g) && aligned16(gw)) go(std::true_type{});
     else go(std::false_type{});
