@@ -183,7 +183,7 @@ fc_soft_bwd_ckpt_kernel(const uint32_t* __restrict__ codes, uint32_t ldw, const 
                 const float half_step = b.x, lo = b.y;
                 const float w = k < K ? S.node.w[j * K + k] : 0.0f;
                 const f32x2 ww = pair(w, w);
-                if (KT > 1) {
+                if (KT > 1 || conn) {       // a single given weight has a gradient too
                     const f32x2 t = fma2(g01, codes2_f32(q[e], 0), mul2(g23, codes2_f32(q[e], 2)));
                     float t0, t1;
                     unpair(t, t0, t1);
@@ -226,7 +226,7 @@ static void launch_ckpt(const FcArgs& A, const uint32_t* codes, int64_t ldw, con
                         float* gx, float* ws, float* gconn, float* gparams, cudaStream_t st) {
     const int64_t nv = A.ldb / 4, nchunk = cdiv(nv, 32 * CB_ITER);
     constexpr int smem = CB_WARPS * (int)sizeof(CkptSmem<NODE, KT>);
-    static_assert(sizeof(CkptSmem<NODE, KT>) % 16 == 0 && 3 * (smem + 1024) <= 227 * 1024 + 512, "five CTAs per SM");
+    static_assert(sizeof(CkptSmem<NODE, KT>) % 16 == 0 && 3 * (smem + 1024) <= 227 * 1024 + 512, "three CTAs per SM");
     if (smem > 48 * 1024)
         cudaFuncSetAttribute(fc_soft_bwd_ckpt_kernel<NODE, KT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     const int npart = 2 * A.K + NodeSize<NODE, 2>::NPG;

@@ -237,3 +237,71 @@ def test_step_on_another_stream_and_in_a_graph():
         x.normal_()
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(kept, both()))
+
+
+def test_equal_rows_tie_across_beams():
+    """Beams with the same logits and scores (a decoder's first steps) have equal candidates: the
+    lowest beam wins, whatever the rows' alignment and the number of beams."""
+    g = torch.Generator().manual_seed(0)
+    for V in (777, 8191, 20001):
+        for k in (3, 5, 8):
+            for dtype in DTYPES:
+                x = (3 * torch.randn(1, V, generator=g)).to(dtype).to(dev).expand(2 * k, V).contiguous()
+                r = S.beam_step(x, torch.full((2, k), -7.0, device=dev))
+                top = x[0].float().max()
+                first = torch.nonzero(x[0].float() == top).flatten()
+                # the best token of every beam ties: beams in order, tokens in order within a beam
+                want = [(b, t) for b in range(k) for t in first.tolist()][:k]
+                for e in range(2):
+                    assert list(zip(r.parents[e].tolist(), r.tokens[e].tolist())) == want
+
+
+def test_large_magnitudes():
+    """Logits far from zero: the normaliser keeps its accuracy (sums run relative to the maximum)."""
+    g = torch.Generator().manual_seed(1)
+    base = 4 * torch.randn(6, 3000, generator=g, dtype=torch.float64)
+    for shift in (0.0, 1000.0, -1000.0, 60000.0, 1e5, -1e6):
+        x = (base + shift).float().to(dev)
+        _check(x, -torch.rand(2, 3, generator=g).to(dev))
+    big = torch.tensor([[1e30, 2e30, 2e30, -3e38]], device=dev)
+    r = S.beam_step(big, torch.zeros(1, 1, device=dev), width=4)
+    assert r.tokens.tolist() == [[1, 2, 0, 3]]
+    assert (r.scores[0, :2] + 0.6931472).abs().max() < 1e-6 and bool((r.scores[0, 2:] < -1e29).all())
+
+
+def test_logits_past_2_31_elements():
+    V = 70_000_000
+    x = torch.full((32, V), -3.0, dtype=torch.bfloat16, device=dev)
+    x[31, V - 1] = 40.0
+    x[30, V - 2] = 39.0
+    r = S.beam_step(x, torch.zeros(1, 32, device=dev), width=2)
+    assert r.parents.tolist() == [[30, 31]] or r.parents.tolist() == [[31, 30]]
+    assert set(r.tokens[0].tolist()) == {V - 1, V - 2}
+
+
+def test_example_trains_and_decodes():
+    import importlib.util
+    import os
+    from conftest import ROOT
+    spec = importlib.util.spec_from_file_location("token_logic_net", os.path.join(ROOT, "examples", "token_logic_net.py"))
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    torch.manual_seed(0)
+    net = ex.TokenLogicNet(12, dim=32, state=128).to(dev)
+    first = ex.train(net, 1, batch_size=128, length=6, log=None)
+    last = ex.train(net, 120, batch_size=128, length=6, log=None)
+    assert last < 0.8 * first
+    prompt = ex.batch(5, 4, 12, torch.Generator().manual_seed(1), dev)
+    tokens, scores = net.generate(prompt, 5, beams=3)
+    assert tokens.shape == (5, 3, 5) and bool((scores[:, :-1] >= scores[:, 1:]).all())
+    # one beam is the greedy decoder of the circuit, step by step
+    tokens, _ = net.generate(prompt, 5, beams=1)
+    step = net.circuit()
+    from silogic_b200.bitpacking import pack_bits
+    h = pack_bits(torch.zeros((5, 128), dtype=torch.uint8, device=dev))
+    for t in range(4):
+        logits, h = step(prompt[:, t].contiguous(), h)
+    for t in range(5):
+        ids = logits.argmax(1)
+        assert torch.equal(ids, tokens[:, 0, t])
+        logits, h = step(ids, h)

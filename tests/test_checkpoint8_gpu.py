@@ -264,3 +264,96 @@ def test_training_step_in_a_cuda_graph():
         step = GraphedTrainStep(net, opt, (128, 64), dev)
         losses = [step.step(x.to(dev), y.to(dev)).item() for _ in range(60)]
     assert step.graph is not None and losses[-1] < 0.7 * losses[0]
+
+
+# -------------------------------------------- the backward that reads codes
+KINDS = {"gate16": (0, 16), "walsh": (1, 4), "multilinear": (2, 4), "hybrid": (3, 4)}
+
+
+@pytest.mark.parametrize("node", list(KINDS))
+@pytest.mark.parametrize("K", [1, 2, 4, 5, 8])
+@pytest.mark.parametrize("B,wire,ste", [(1, 0, 0), (4, 7, 0), (131, 0, 1), (1020, 33, 0), (1028, 0, 2), (4500, 0, 0)])
+def test_backward_from_codes_matches_the_restored_one(node, K, B, wire, ste):
+    """The fused kernel against the fp32 kernel on the values read back (the same sums in
+    another order: the tolerance of the layers' gradient tests)."""
+    from silogic_b200._ops import IMPL
+    kind, npar = KINDS[node]
+    I, O = 61, 75
+    g = torch.Generator().manual_seed(B + K)
+    ldb = _soft.ldb_for(B)
+    xt = torch.zeros(I, ldb)
+    xt[:, :B] = torch.rand(I, B, generator=g)
+    gy = torch.zeros(O, ldb)
+    gy[:, :B] = torch.randn(O, B, generator=g)
+    cand = torch.randint(0, I, (O, 2, K), generator=g, dtype=torch.int32).to(dev)
+    conn = torch.randn(O, 2, K, generator=g).to(dev) if K > 1 or ste == 2 else None
+    params = torch.randn(O, npar, generator=g).to(dev)
+    xt, gy = xt.to(dev), gy.to(dev)
+    codes, bounds = IMPL["ckpt_store"](xt[:, :B])
+    args = (K, ste, kind, 2, 0, 1.3 if node == "walsh" else 1.0, O, wire)
+    got = IMPL["fc_soft_bwd_ckpt"](codes, bounds, ldb, cand, conn, params, *args, gy, True)
+    seen = torch.zeros_like(xt)
+    seen[:, :B] = IMPL["ckpt_load"](codes, bounds, B, torch.float32)
+    want = IMPL["fc_soft_bwd"](seen, cand, conn, params, *args, gy, True)
+    for a, b, what in zip(got, want, ("x", "parameters", "connections")):
+        if b.numel():
+            _close(a[:, :B] if what == "x" else a, (b[:, :B] if what == "x" else b).double(), what)
+    again = IMPL["fc_soft_bwd_ckpt"](codes, bounds, ldb, cand, conn, params, *args, gy, False)
+    assert again[0].numel() == 0 and torch.equal(again[1], got[1]) and torch.equal(again[2], got[2])
+
+
+def test_blocks_that_are_not_finite_reach_the_gradients():
+    layer = S.LogicLayer(20, 30, node="walsh", k=4, seed=0).to(dev)
+    x = torch.rand(256, 20, device=dev)
+    x[3, 7] = float("nan")
+    x.requires_grad_(True)
+    with S.checkpoint8():
+        y = layer(x)
+    gx, gp = torch.autograd.grad(y, [x, layer.node.param], torch.ones_like(y))
+    reads = (layer._conn.cand == 7).any(2).any(1)
+    assert bool(torch.isnan(gp[reads]).all()) and not bool(torch.isnan(gp[~reads]).any())
+    assert bool(torch.isnan(gx[:128]).any()) and not bool(torch.isnan(gx[128:]).any())
+
+
+def test_offsets_past_32_bits():
+    """4.3e9 activations: codes and gradient rows beyond 2^32 bytes and elements."""
+    from silogic_b200._ops import IMPL
+    I, B, K = 8300, 524288, 2
+    codes = torch.randint(0, 256, (I, B), dtype=torch.uint8, device=dev)
+    bounds = torch.rand(I, B // 128, 2, device=dev) * 0.01
+    cand = torch.tensor([[[I - 1, 5], [I - 2, I - 1]]], dtype=torch.int32, device=dev)
+    conn, params = torch.randn(1, 2, K, device=dev), torch.randn(1, 4, device=dev)
+    gy = torch.randn(1, B, device=dev)
+    args = (K, 0, 1, 2, 0, 1.0, 1, 0)
+    gx, gp, gc = IMPL["fc_soft_bwd_ckpt"](codes, bounds, B, cand, conn, params, *args, gy, True)
+    rows = torch.tensor([5, I - 2, I - 1], device=dev)
+    small = torch.tensor([[[2, 0], [1, 2]]], dtype=torch.int32, device=dev)
+    seen = IMPL["ckpt_load"](codes[rows].contiguous(), bounds[rows].contiguous(), B, torch.float32)
+    wx, wp, wc = IMPL["fc_soft_bwd"](seen, small, conn, params, *args, gy, True)
+    _close(gx[rows], wx.double(), "x")
+    _close(gp, wp.double(), "parameters")
+    _close(gc, wc.double(), "connections")
+    assert not bool((gx[6:I - 2:97] != 0).any())
+    del gx
+    x = IMPL["ckpt_load"](codes, bounds, B, torch.bfloat16)
+    assert torch.equal(x[rows], seen.to(torch.bfloat16))
+    back, b2 = IMPL["ckpt_store"](x)
+    assert torch.equal(back[rows], IMPL["ckpt_store"](x[rows])[0]) and torch.equal(b2[rows], IMPL["ckpt_store"](x[rows])[1])
+
+
+def test_a_net_of_checkpointed_layers_traces_under_torch_compile():
+    torch.manual_seed(0)
+    net = S.LogicNet(40, 60, 2, node="walsh", k=4, tau=3.0, seed=0).to(dev)
+    x = torch.rand(50, 40, device=dev)
+
+    def grads(f):
+        net.zero_grad()
+        with S.checkpoint8():
+            out = f(x)
+        (out * torch.arange(10, device=dev)).sum().backward()
+        return out.detach(), [p.grad.clone() for p in net.parameters()]
+    y0, g0 = grads(net)
+    y1, g1 = grads(torch.compile(net, backend="aot_eager", fullgraph=True))
+    assert torch.equal(y0, y1)
+    for a, b in zip(g0, g1):
+        _close(a, b.double(), "compiled")

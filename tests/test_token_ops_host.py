@@ -96,3 +96,37 @@ def test_c_entry_points_refuse_bad_arguments(L):
     assert L.slg_beam_reorder_features(_p(256), 3, 7, _p(256), 2, 4, 4, _p(512), 8, _p(0)) == 1       # rows too short
     assert L.slg_beam_reorder_features(_p(256), 3, 8, _p(256), 2, 4, 4, _p(512), 7, _p(0)) == 1
     assert L.slg_beam_reorder_packed(_p(256), 3, 1, _p(256), 20, 4, 4, _p(512), 2, _p(0)) == 1
+
+
+def test_checkpoint_backward_refuses_bad_arguments(L):
+    need = L.slg_fc_soft_workspace_bytes(512, 8, 1, 2, 100)
+    ok = dict(codes=256, ldc=512, bounds=256, I=50, ldb=512, cand=256, conn=256, K=8, ste=0, node=1, ar=2, par=256,
+              O=100, wire=0, gy=256, gx=256, gconn=256, gpar=256, ws=256, size=need)
+
+    def call(**k):
+        a = dict(ok, **k)
+        return L.slg_fc_soft_bwd_ckpt(_p(a["codes"]), a["ldc"], _p(a["bounds"]), a["I"], a["ldb"], _p(a["cand"]),
+                                      _p(a["conn"]), a["K"], a["ste"], a["node"], a["ar"], _p(a["par"]), 0, 1.0, a["O"],
+                                      a["wire"], _p(a["gy"]), _p(a["gx"]), _p(a["gconn"]), _p(a["gpar"]), _p(a["ws"]),
+                                      a["size"], _p(0))
+    assert call(I=0) == 1 and call(ldb=0) == 1 and call(K=0) == 1 and call(wire=-1) == 1 and call(O=-1) == 1
+    assert call(K=9) == 3 and call(ar=3) == 3 and call(node=4) == 3                # restore instead
+    assert call(ldb=510) == 2 and call(ldc=514) == 2 and call(ldc=508) == 1
+    assert call(ste=3) == 1 and call(wire=51) == 1 and call(wire=101) == 1
+    for name in ("codes", "bounds", "cand", "par", "gy", "gpar", "ws", "gconn"):
+        assert call(**{name: 0}) == 1, name
+    assert call(gy=264) == 2 and call(gx=264) == 2 and call(codes=258) == 2 and call(bounds=260) == 2
+    assert call(size=need - 1) == 5
+    assert call(O=0) == 0
+    for K, node, ar, want in ((8, 0, 2, 1), (1, 3, 2, 1), (9, 0, 2, 0), (4, 1, 3, 0), (4, 4, 2, 0), (4, 5, 2, 0), (0, 1, 2, 0)):
+        assert L.slg_fc_soft_bwd_ckpt_built(K, node, ar) == want
+
+
+@pytest.mark.parametrize("beams", [1, 2, 3, 5, 7, 8, 16, 31, 32])
+def test_packed_reorder_sources_lie_in_four_words(beams):
+    """The kernel that loads four source words per output word (width >= beams) relies on it."""
+    for width in range(beams, 33):
+        for word in range(0, 6 * width):
+            first = (word * 32 // width * beams) >> 5
+            last = ((word * 32 + 31) // width) * beams + beams - 1
+            assert last - 32 * first < 128

@@ -176,3 +176,45 @@ def test_module_trains_and_keeps_its_padding_row():
     ids[0] = 3
     m(ids).sum().backward()
     assert bool((m.weight.grad[3] == 0).all()) and bool((m.weight.grad != 0).any())
+
+
+def test_offsets_past_32_bits():
+    """A table of 2.6e9 values: rows, gradients and carries beyond 2^32 bytes and 2^31 elements."""
+    V, D = 50000, 52000
+    w = torch.zeros(V, D, dtype=torch.bfloat16, device=dev)
+    w[V - 1] = 3.0
+    w[V - 2, D - 1] = 5.0
+    w.requires_grad_(True)
+    ids = torch.tensor([V - 1, 0, V - 2, V - 1], device=dev)
+    y = S.token_embedding(ids, w, scale=2.0)
+    assert bool((y[0] == 6).all()) and bool((y[1] == 0).all()) and y[2, D - 1] == 10 and bool((y[3] == 6).all())
+    gy = torch.ones(4, D, dtype=torch.bfloat16, device=dev)
+    (gw,) = torch.autograd.grad(y, w, gy)
+    assert bool((gw[V - 1] == 4).all()) and bool((gw[V - 2] == 2).all()) and bool((gw[0] == 2).all())
+    assert not bool((gw[1:V - 2] != 0).any())
+
+
+@pytest.mark.parametrize("N,V,top", [(20000, 50, 0.9), (60000, 30000, 0.5), (140000, 65536, 0.3)])
+def test_rows_cut_into_many_chunks(N, V, top):
+    """Frequent tokens whose rows span hundreds of chunks beside many rows that span two."""
+    g = torch.Generator().manual_seed(N)
+    ids = torch.randint(0, V, (N,), generator=g)
+    ids[torch.rand(N, generator=g) < top] = V // 2
+    for D, dtype in ((136, torch.float32), (264, torch.bfloat16), (130, torch.float16), (600, torch.float32)):
+        ids_d, w, gy = _case(V, D, N, dtype, ids=ids)
+        w.requires_grad_(True)
+        (gw,) = torch.autograd.grad(S.token_embedding(ids_d, w), w, gy)
+        _check_grad(gw, ids_d, gy, V, 1.0)
+
+
+def test_traced_by_torch_compile():
+    """Lookup and gradient are torch.library ops with fake implementations: no graph break."""
+    m = S.TokenEmbedding(100, 24, padding_idx=0).to(dev)
+    ids = torch.randint(0, 100, (6, 7), device=dev)
+    f = torch.compile(lambda i: (m(i) ** 2).sum(), backend="aot_eager", fullgraph=True)
+    m.zero_grad()
+    f(ids).backward()
+    got = m.weight.grad.clone()
+    m.zero_grad()
+    (m(ids) ** 2).sum().backward()
+    assert torch.equal(got, m.weight.grad)
