@@ -385,6 +385,11 @@ int slg_ckpt_store(const void* x, int32_t dtype, int64_t rows, int64_t cols, int
                    uint8_t* codes, int64_t ldc, float* bounds, void* stream);
 int slg_ckpt_load(const uint8_t* codes, int64_t ldc, const float* bounds, int64_t rows,
                   int64_t cols, void* x, int32_t dtype, int64_t ldx, void* stream);
+/* slg_to_feature_major and slg_ckpt_store of its result's first B columns in one pass over
+ * x [B, F]: out [F, ldb], codes [F, ldc] (ldc >= ldb), bounds [F, ceil(B /
+ * SLG_CKPT_BLOCK), 2]; ldb may not reach past the last block. */
+int slg_to_feature_major_ckpt(const float* x, int64_t B, int64_t F, float* out, int64_t ldb,
+                              uint8_t* codes, int64_t ldc, float* bounds, void* stream);
 
 /* slg_fc_soft_bwd with the layer's input read from an 8-bit checkpoint of its
  * feature-major activations: codes [in_dim, ldc], bounds [in_dim,

@@ -60,6 +60,7 @@ _SIGS = {
     "slg_embed_bwd": [_p, _i32, _i64, _p, _i32, _i64, _i64, _f32, _i64, _p, _p, _i64, _p],
     "slg_ckpt_store": [_p, _i32, _i64, _i64, _i64, _p, _i64, _p, _p],
     "slg_ckpt_load": [_p, _i64, _p, _i64, _i64, _p, _i32, _i64, _p],
+    "slg_to_feature_major_ckpt": [_p, _i64, _i64, _p, _i64, _p, _i64, _p, _p],
     "slg_fc_soft_bwd_ckpt": [_p, _i64, _p, _i64, _i64, _p, _p, _i32, _i32, _i32, _i32, _p, _i32,
                              _f32, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p],
     "slg_beam_step": [_p, _i32, _i64, _i32, _i64, _i64, _p, _p, _i32, _i32, _p, _p, _p, _p, _p],

@@ -369,6 +369,28 @@ def _(codes, bounds, cols, dtype):
     return codes.new_empty((codes.shape[0], cols), dtype=dtype)
 
 
+@_op("to_feature_major_ckpt")
+def to_feature_major_ckpt(x: Tensor, ldb: int) -> Tuple[Tensor, Tensor, Tensor]:
+    """``[B, F]`` -> (feature-major ``[F, ldb]`` fp32, codes, bounds) in one pass."""
+    require_cuda(x)
+    x = x.float().contiguous()
+    B, F = x.shape
+    out = x.new_empty((F, ldb))
+    codes = x.new_empty((F, (ldb + 15) // 16 * 16), dtype=torch.uint8)
+    bounds = x.new_empty((F, -(-B // CKPT_BLOCK), 2))
+    call("slg_to_feature_major_ckpt", x.data_ptr(), B, F, out.data_ptr(), ldb, codes.data_ptr(),
+         codes.shape[1], bounds.data_ptr(), stream_ptr(x.device))
+    return out, codes, bounds
+
+
+@to_feature_major_ckpt.register_fake
+def _(x, ldb):
+    B, F = x.shape
+    return (x.new_empty((F, ldb), dtype=torch.float32),
+            x.new_empty((F, (ldb + 15) // 16 * 16), dtype=torch.uint8),
+            x.new_empty((F, (B + CKPT_BLOCK - 1) // CKPT_BLOCK, 2), dtype=torch.float32))
+
+
 @_op("fc_soft_bwd_ckpt")
 def fc_soft_bwd_ckpt(codes: Tensor, bounds: Tensor, ldb: int, cand: Tensor, conn: Optional[Tensor],
                      params: Tensor, K: int, ste: int, node: int, arity: int, gate_hard: int,

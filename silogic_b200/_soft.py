@@ -115,15 +115,16 @@ class FCSoft(torch.autograd.Function):
                 float(meta["inv_tau"]), meta["out_dim"], meta["wire_r"])
 
     @staticmethod
-    def forward(ctx, xt, params, conn, meta):
+    def forward(ctx, xt, params, conn, meta, kept=None):
+        """``kept``: the checkpoint (codes, bounds) of ``xt`` where it was stored already."""
         require_cuda(xt)
         xt = xt.contiguous()
         params = params.float().contiguous()
         connc = conn.float().contiguous() if conn is not None else None
         y = op("fc_soft_fwd")(xt, meta["cand"], connc, params, *FCSoft._args(meta))
-        ctx.ckpt = _keep_checkpoint(ctx)
+        ctx.ckpt = kept is not None or _keep_checkpoint(ctx)
         if ctx.ckpt:        # the backward pass works from 8-bit codes; xt itself is let go
-            ctx.save_for_backward(*_store(xt, meta), params, connc)
+            ctx.save_for_backward(*(kept or _store(xt, meta)), params, connc)
             ctx.ldb = xt.shape[1]
         else:
             ctx.save_for_backward(xt, params, connc)
@@ -161,8 +162,12 @@ class FCSoftRows(torch.autograd.Function):
     def forward(ctx, x, params, conn, meta):
         ctx.shape = x.shape
         B = x.shape[0]
-        xt = op("to_feature_major")(x.reshape(B, -1), ldb_for(B))
-        return op("from_feature_major")(FCSoft.forward(ctx, xt, params, conn, meta), B)
+        x, kept = x.reshape(B, -1), None
+        if B and _keep_checkpoint(ctx):
+            xt, *kept = op("to_feature_major_ckpt")(x, ldb_for(B))
+        else:
+            xt = op("to_feature_major")(x, ldb_for(B))
+        return op("from_feature_major")(FCSoft.forward(ctx, xt, params, conn, meta, kept), B)
 
     @staticmethod
     def backward(ctx, gy):

@@ -16,7 +16,6 @@ BEAM_MAX = 32           # SLG_BEAM_MAX
 BeamStep = namedtuple("BeamStep", "scores parents tokens finished")
 
 
-@torch.no_grad()
 def beam_step(logits, scores, finished=None, eos=None, width=None):
     """The ``width`` (default: as many as there are) best continuations of each entry's beams.
 
@@ -36,7 +35,8 @@ def beam_step(logits, scores, finished=None, eos=None, width=None):
         raise ValueError(f"beam_step: vocabulary of {V} (must be below 2**27)")
     if logits.shape != (B * beams, V) and logits.shape != (B, beams, V):
         raise ValueError(f"beam_step: logits {tuple(logits.shape)} do not fit scores {tuple(scores.shape)}")
-    require_cuda(logits, scores, finished)
+    if not (logits.is_cuda and scores.is_cuda and (finished is None or finished.is_cuda)):
+        require_cuda(logits, scores, finished)
     width = beams if width is None else int(width)
     if not 1 <= beams <= BEAM_MAX or not 1 <= width <= BEAM_MAX:
         raise ValueError(f"beam_step: beams and width must be in 1..{BEAM_MAX}, got {beams} and {width}")
@@ -54,10 +54,9 @@ def beam_step(logits, scores, finished=None, eos=None, width=None):
     x = logits if logits.dim() == 2 else logits.reshape(B * beams, V)
     if B and (x.stride(1) != 1 and V > 1 or x.stride(0) < V):
         x = x.contiguous()
-    scores = scores.float().contiguous()
+    scores = scores.detach().float().contiguous()
     out = scores.new_empty((B, width))
-    parents = scores.new_empty((B, width), dtype=torch.int64)
-    tokens = torch.empty_like(parents)
+    parents, tokens = scores.new_empty((2, B, width), dtype=torch.int64).unbind(0)
     done = scores.new_empty((B, width), dtype=torch.bool) if eos is not None else None
     call("slg_beam_step", x.data_ptr(), DTYPE_ID[x.dtype], B, beams, V, max(x.stride(0), V), scores.data_ptr(),
          ptr(finished), -1 if eos is None else int(eos), width, out.data_ptr(), parents.data_ptr(),
@@ -65,7 +64,6 @@ def beam_step(logits, scores, finished=None, eos=None, width=None):
     return BeamStep(out, parents, tokens, done)
 
 
-@torch.no_grad()
 def beam_reorder(state, parents, layout="rows", beams=None):
     """The decoder state after a step: sample ``e * width + n`` is the state's sample
     ``e * beams + parents[e, n]``, for ``parents`` ``[B, width]`` of :func:`beam_step`.
@@ -76,11 +74,12 @@ def beam_reorder(state, parents, layout="rows", beams=None):
     the number of beams that the state holds per entry."""
     if parents.dim() != 2 or parents.dtype != torch.int64:
         raise ValueError("beam_reorder: parents must be [B, width] int64")
-    require_cuda(state, parents)
+    if not (state.is_cuda and parents.is_cuda):
+        require_cuda(state, parents)
     B, width = parents.shape
     parents = parents.contiguous()
     st = stream_ptr(state.device)
-    state = state.contiguous()
+    state = state.detach().contiguous()
     if layout == "rows":
         if beams is None:
             beams = state.shape[0] // B if B else width
@@ -88,7 +87,7 @@ def beam_reorder(state, parents, layout="rows", beams=None):
             raise ValueError(f"beam_reorder: {tuple(state.shape)} does not hold {B} entries of {beams} beams")
         out = state.new_empty((B * width,) + tuple(state.shape[1:]))
         nbytes = out.numel() * out.element_size() // (B * width) if B else 0
-        call("slg_beam_reorder_rows", ptr(state), nbytes, ptr(parents), B, beams, width, ptr(out), st)
+        call("slg_beam_reorder_rows", state.data_ptr(), nbytes, parents.data_ptr(), B, beams, width, out.data_ptr(), st)
         return out
     beams = width if beams is None else int(beams)
     if layout == "features":
@@ -103,5 +102,5 @@ def beam_reorder(state, parents, layout="rows", beams=None):
     if beams < 1 or ld * size < B * beams:
         raise ValueError(f"beam_reorder: rows of {ld} do not hold {B} entries of {beams} beams")
     out = torch.empty_like(state) if beams == width else state.new_empty((F, ld_for(B * width)))
-    call(fn, ptr(state), F, ld, ptr(parents), B, beams, width, ptr(out), out.shape[1], st)
+    call(fn, state.data_ptr(), F, ld, parents.data_ptr(), B, beams, width, out.data_ptr(), out.shape[1], st)
     return out

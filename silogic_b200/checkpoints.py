@@ -31,24 +31,26 @@ class Checkpoint8:
         dtype = dtype or self.dtype
         if dtype not in DTYPE_ID:
             raise TypeError(f"restore: dtype must be float32, bfloat16 or float16, got {dtype}")
-        if self.shape.numel() == 0:
-            return torch.empty(self.shape, dtype=dtype, device=self.codes.device)
-        return op("ckpt_load")(self.codes, self.bounds, self.shape[-1], dtype).view(self.shape)
+        shape = self.shape
+        if shape.numel() == 0:
+            return torch.empty(shape, dtype=dtype, device=self.codes.device)
+        out = op("ckpt_load")(self.codes, self.bounds, shape[-1], dtype)
+        return out if len(shape) == 2 else out.view(shape)
 
     def nbytes(self):
         return self.codes.numel() + 4 * self.bounds.numel()
 
 
-@torch.no_grad()
 def checkpoint8_store(x):
     """Keep ``x`` (float32, bfloat16 or float16, at least one dimension) in 8 bits: each run
     of 128 values along the last dimension is cut into 255 steps between its smallest and
     its largest value.  A run that holds a NaN or an infinity reads back as NaN."""
-    require_cuda(x)
     if x.dtype not in DTYPE_ID:
         raise TypeError(f"checkpoint8_store: x must be float32, bfloat16 or float16, got {x.dtype}")
     if x.dim() == 0:
         raise ValueError("checkpoint8_store: x must have at least one dimension")
+    require_cuda(x)
+    x = x.detach()
     if x.numel() == 0:
         rows, cols = 0, x.shape[-1]
         return Checkpoint8(torch.empty((rows, cols), dtype=torch.uint8, device=x.device),

@@ -181,6 +181,81 @@ ckpt_load_kernel(const uint32_t* __restrict__ codes, int64_t ldw, const float2* 
     }
 }
 
+// Rows [B, F] -> feature-major [F, ldb] (columns >= B zero) and its checkpoint in one pass: a
+// CTA holds 32 features x 128 samples, one block of each feature, so the codes cost no
+// second read of the activations.  Lane l has samples l, l + 32, ...: reads and writes of
+// the tile are free of bank conflicts, and codes are stored byte by byte in whole lines.
+constexpr int TC_F = 32;
+template <bool WHOLE>       // the tile lies inside [B, F]: no bounds checks
+__device__ __forceinline__ void to_fm_ckpt_tile(const float* __restrict__ x, int64_t B, int64_t F, float* __restrict__ out,
+                                                int64_t ldb, uint8_t* __restrict__ codes, int64_t ldc,
+                                                float2* __restrict__ bounds, int64_t nblk,
+                                                float (&t)[TC_F][CK_BLOCK + 1]) {
+    constexpr int ROWS = TC_F / 8;              // features per warp
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t f0 = (int64_t)blockIdx.x * TC_F, blk = blockIdx.y, b0 = blk * CK_BLOCK;
+    {
+        float v[16];
+        const float* p = x + (b0 + warp) * F + f0 + lane;
+#pragma unroll
+        for (int i = 0; i < 16; ++i, p += 8 * F)
+            v[i] = WHOLE || (b0 + warp + 8 * i < B && f0 + lane < F) ? __ldg(p) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t[lane][warp + 8 * i] = v[i];
+    }
+    __syncthreads();
+    const int left = (int)(B - b0 < CK_BLOCK ? B - b0 : CK_BLOCK);          // samples of the tile
+    const int width = (int)(ldb - b0 < CK_BLOCK ? ldb - b0 : CK_BLOCK);     // its columns
+    const int64_t f = f0 + warp * ROWS;
+    float lo[ROWS], my_lo = 0.0f, my_range = 0.0f;
+    float* o = out + f * ldb + b0 + lane;
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u, o += ldb) {
+        float l = CUDART_INF_F, h = -CUDART_INF_F;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float v = t[warp * ROWS + u][lane + 32 * j];
+            if (WHOLE || lane + 32 * j < left) {
+                l = fminf(l, v);
+                h = max_nan_f32(h, v);
+            }
+            if (WHOLE || (f + u < F && lane + 32 * j < width)) o[32 * j] = v;
+        }
+        lo[u] = warp_min_f32(l);
+        const float range = __fsub_rn(warp_max_nan_f32(h), lo[u]);
+        if (lane == u) { my_lo = lo[u]; my_range = range; }
+    }
+    const bool bad = !isfinite(my_range);
+    const float step = __fmul_rn(my_range, 1.0f / 255.0f);
+    const bool flat = bad || step < CK_TINY;
+    const float my_inv = flat ? 0.0f : __fdiv_rn(255.0f, my_range);
+    if (lane < ROWS && f + lane < F)
+        bounds[(f + lane) * nblk + blk] =
+            bad ? make_float2(CUDART_NAN_F, CUDART_NAN_F) : make_float2(my_lo, flat ? 0.0f : step);
+    uint8_t* c = codes + f * ldc + b0 + lane;
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u, c += ldc) {
+        const float inv = __shfl_sync(0xffffffffu, my_inv, u);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t code = __float_as_uint(
+                __fadd_rn(__fmul_rn(__fsub_rn(t[warp * ROWS + u][lane + 32 * j], lo[u]), inv), 12582912.0f));
+            if (WHOLE) c[32 * j] = (uint8_t)(inv != 0.0f ? code : 0u);
+            else if (f + u < F && lane + 32 * j < width)
+                c[32 * j] = (uint8_t)(lane + 32 * j < left && inv != 0.0f ? code : 0u);
+        }
+    }
+}
+
+__global__ void __launch_bounds__(256, 5)
+to_fm_ckpt_kernel(const float* __restrict__ x, int64_t B, int64_t F, float* __restrict__ out, int64_t ldb,
+                  uint8_t* __restrict__ codes, int64_t ldc, float2* __restrict__ bounds, int64_t nblk) {
+    __shared__ float t[TC_F][CK_BLOCK + 1];
+    if (((int64_t)blockIdx.x + 1) * TC_F <= F && ((int64_t)blockIdx.y + 1) * CK_BLOCK <= B)
+        to_fm_ckpt_tile<true>(x, B, F, out, ldb, codes, ldc, bounds, nblk, t);
+    else to_fm_ckpt_tile<false>(x, B, F, out, ldb, codes, ldc, bounds, nblk, t);
+}
+
 static int check_ckpt(const void* codes, int64_t ldc, const void* bounds, int64_t rows, int64_t cols, int64_t ldx,
                       int dtype, const char* name) {
     if (rows < 0 || cols < 0) return set_error(SLG_ERR_ARG, "%s: bad sizes", name);
@@ -235,4 +310,21 @@ extern "C" int slg_ckpt_load(const uint8_t* codes, int64_t ldc, const float* bou
             nblk, (T*)x, ldx, vec);
     });
     return check_launch("slg_ckpt_load");
+}
+
+extern "C" int slg_to_feature_major_ckpt(const float* x, int64_t B, int64_t F, float* out, int64_t ldb, uint8_t* codes,
+                                         int64_t ldc, float* bounds, void* stream) {
+    const char* name = "slg_to_feature_major_ckpt";
+    if (B <= 0 || F < 0 || ldb < B || ldc < ldb) return set_error(SLG_ERR_ARG, "%s: bad sizes", name);
+    const int64_t nblk = cdiv(B, CK_BLOCK);
+    // one tile row per block: padding columns may not begin another block
+    if (cdiv(ldb, CK_BLOCK) != nblk) return set_error(SLG_ERR_ARG, "%s: ldb reaches past the last block", name);
+    if (nblk > 65535) return set_error(SLG_ERR_ARG, "%s: batch too large", name);
+    if (F == 0) return SLG_OK;
+    if (!x || !out || !codes || !bounds) return set_error(SLG_ERR_ARG, "%s: null pointer", name);
+    if (!aligned_to(bounds, 8)) return set_error(SLG_ERR_ALIGN, "%s: bounds misaligned", name);
+    const dim3 grid((unsigned)cdiv(F, TC_F), (unsigned)nblk);
+    to_fm_ckpt_kernel<<<grid, 256, 0, as_stream(stream)>>>(x, B, F, out, ldb, codes, ldc,
+                                                           reinterpret_cast<float2*>(bounds), nblk);
+    return check_launch(name);
 }

@@ -357,3 +357,21 @@ def test_a_net_of_checkpointed_layers_traces_under_torch_compile():
     assert torch.equal(y0, y1)
     for a, b in zip(g0, g1):
         _close(a, b.double(), "compiled")
+
+
+@pytest.mark.parametrize("B,F", [(1, 1), (3, 70), (5, 64), (127, 65), (128, 63), (130, 200), (1000, 333), (4093, 90)])
+def test_transpose_and_store_in_one_pass(B, F):
+    """Bit for bit the transpose followed by the store of its first B columns."""
+    from silogic_b200._ops import IMPL
+    g = torch.Generator().manual_seed(B)
+    x = torch.randn(B, F, generator=g)
+    x[:, 0] = 0.75
+    if F > 2:
+        x[B // 2, 1], x[0, 2] = float("nan"), float("inf")
+    x = x.to(dev)
+    ldb = _soft.ldb_for(B)
+    out, codes, bounds = IMPL["to_feature_major_ckpt"](x, ldb)
+    want = IMPL["to_feature_major"](x, ldb)
+    wc, wb = IMPL["ckpt_store"](want[:, :B])
+    eq = lambda a, b: torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))       # noqa: E731
+    assert eq(out, want) and eq(bounds, wb) and torch.equal(codes[:, :ldb], wc[:, :ldb])
