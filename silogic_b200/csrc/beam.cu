@@ -21,6 +21,7 @@ constexpr int BM_WARPS = BM_THREADS / 32;
 constexpr int BM_PER = 32;              // logits a lane holds at once
 constexpr int BM_UNIT = 32 * BM_PER;    // logits of one unit of a warp's work
 constexpr int BM_MAX = SLG_BEAM_MAX;
+static_assert(BM_WARPS * BM_MAX <= BM_THREADS, "the join gives every winner a thread");
 constexpr float BM_LARGEST = 3.402823466e+38f;
 
 // NaN -> -inf, +inf -> the largest finite value (fmaxf returns its other argument for NaN)
@@ -102,9 +103,11 @@ __host__ __device__ inline int beam_parts(int cs, int beams, int units) {
     const int p = cs * BM_WARPS / beams;
     return p < 1 ? 1 : p < units ? p : units;
 }
-// at most 39 KB (8 CTAs, 32 beams, width 32)
+// at most 38,144 bytes (8 CTAs, 32 beams, width 32) beside the warps' 8,448 of scratch
+constexpr int BM_LIST = 34;             // candidates and a 0 before a warp's list in its scratch
+constexpr int BM_SCRATCH = BM_LIST + 32;
 static inline size_t beam_smem(int items, int beams, int width) {
-    return (size_t)items * (width * 8 + 8) + (size_t)BM_WARPS * width * 8 + beams * 8;
+    return (size_t)(items * width + (items * width & 1)) * 8 + (size_t)BM_WARPS * width * 8 + (size_t)items * 8 + beams * 8;
 }
 
 // logits [at, at + E) of a row of V, masked past its end
@@ -131,7 +134,9 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
                  const uint8_t* __restrict__ finished, int32_t eos, int width, float* __restrict__ out_scores,
                  int64_t* __restrict__ parents, int64_t* __restrict__ tokens, uint8_t* __restrict__ out_finished) {
     constexpr int E = Pack16<T>::E;
-    extern __shared__ uint64_t smem[];
+    extern __shared__ __align__(16) uint64_t smem[];
+    __shared__ __align__(16) uint64_t scratches[BM_WARPS][BM_SCRATCH];
+    __shared__ uint32_t floors[BM_WARPS];       // per beam of the CTA: `width` logits of it reach this
     cg::cluster_group cluster = cg::this_cluster();
     const int cs = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -139,18 +144,24 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
     const int parts = beam_parts(cs, beams, units), items = beams * parts;
     BeamSlots own;
     own.key = smem;
-    uint64_t* best = own.key + (size_t)items * width;               // [warps][width]
+    uint64_t* best = own.key + items * width + (items * width & 1); // [warps][width]
     own.m = reinterpret_cast<float*>(best + BM_WARPS * width);
     own.s = own.m + items;
     float* beam_m = own.s + items;                                  // [beams] maximum, log of the sum
     float* beam_l = beam_m + beams;
 
+    uint64_t* scratch = scratches[warp];
+    if (threadIdx.x < BM_WARPS) floors[threadIdx.x] = 0;
+    __syncthreads();
     auto started = cluster.barrier_arrive();                        // the first CTA's memory is there
     bool waited = false;
     for (int item = rank * BM_WARPS + warp; item < items; item += cs * BM_WARPS) {
         const int b = item / parts, part = item - b * parts;
         const int64_t row_at = entry * beams + b;
         const bool done = finished && finished[row_at];
+        // the warps of a beam share its floor (with one part per beam a warp has its own)
+        volatile uint32_t* floor = &floors[parts > 1 ? b - rank * BM_WARPS / parts : warp];
+        if (parts == 1) *floor = 0;
         uint64_t list = 0;                                          // lane i: the i-th best so far
         float m = -CUDART_INF_F, s = 0.0f;
         if (done) {
@@ -193,16 +204,21 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
                     for (int i = 0; i < BM_PER; ++i) t += exp_fast(x[i] - ref);
                     s = fmaf(t, factor, s);
                 }
-                // Logits that can enter the list beat its last entry; while it is being filled,
-                // also the `width`-th largest of the lanes' maxima (so many logits reach that).
+                // Logits that can be among the beam's best reach the last entry of any of its
+                // warps' lists; while a list is being filled, also the `width`-th largest of
+                // the lanes' maxima (so many logits reach that).
                 uint64_t bar = __shfl_sync(0xffffffffu, list, width - 1);
-                if (!__any_sync(0xffffffffu, valid && ordered(top) >= (uint32_t)(bar >> 32))) continue;
-                uint32_t reach = (uint32_t)(bar >> 32);
+                uint32_t reach = max((uint32_t)(bar >> 32), *floor);
+                if (!__any_sync(0xffffffffu, valid && ordered(top) >= reach)) continue;
                 if (bar == 0) {
-                    uint32_t t = valid ? ordered(top) : 0u;
+                    uint32_t t = valid ? ordered(top) : 0u, low = 0;
                     for (int n = 0; n < width; ++n) {
-                        reach = __reduce_max_sync(0xffffffffu, t);
-                        if (lane == __ffs(__ballot_sync(0xffffffffu, t == reach)) - 1) t = 0;
+                        low = __reduce_max_sync(0xffffffffu, t);
+                        if (lane == __ffs(__ballot_sync(0xffffffffu, t == low)) - 1) t = 0;
+                    }
+                    if (low > reach) {
+                        reach = low;
+                        if (lane == 0) atomicMax(const_cast<uint32_t*>(floor), low);
                     }
                 }
                 const float least = reach ? unordered(reach) : -CUDART_INF_F;
@@ -210,8 +226,8 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
 #pragma unroll
                 for (int i = 0; i < BM_PER; ++i) left |= x[i] >= least ? 1u << i : 0u;
                 left &= valid;
-                // the few that qualify are read again (from L1) and inserted one by one: short
-                // code, because a step of few beams mostly waits for instructions
+                // the few that qualify are read again (from L1): short code, because a step of
+                // few beams mostly waits for instructions
                 while (__any_sync(0xffffffffu, left != 0)) {
                     uint64_t k = 0;
                     if (left) {
@@ -220,15 +236,35 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
                         const int64_t at = base + (i / E) * 32 * E + i % E;
                         k = cand_key(clean(to_f32(row[at])), (uint32_t)at);
                     }
-                    for (uint32_t in = __ballot_sync(0xffffffffu, k > bar); in; in &= in - 1) {
-                        const uint64_t w = __shfl_sync(0xffffffffu, k, __ffs(in) - 1);
-                        if (w <= bar) continue;
-                        const int at = __popc(__ballot_sync(0xffffffffu, lane < width && list > w));
-                        const uint64_t up = __shfl_up_sync(0xffffffffu, list, 1);
-                        if (lane < width && lane >= at) list = lane == at ? w : up;
-                        bar = __shfl_sync(0xffffffffu, list, width - 1);
+                    const uint32_t in = __ballot_sync(0xffffffffu, k > bar);
+                    if (in == 0) continue;
+                    // the place of every candidate and every list entry is the number of keys
+                    // that beat it: all are counted side by side (inserted one by one, each
+                    // waits for the one before)
+                    const int count = __popc(in);
+                    if (k > bar) scratch[__popc(in & ((1u << lane) - 1u))] = k;
+                    if (lane == 0) scratch[count] = 0;
+                    scratch[BM_LIST + lane] = list;
+                    __syncwarp();
+                    int place = 0, moved = lane;
+                    for (int j = 0; j < count; j += 2) {
+                        const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(scratch + j);
+                        place += (w.x > k) + (w.y > k);
+                        moved += (w.x > list) + (w.y > list);
                     }
+                    for (int j = 0; j < width; j += 2) {
+                        const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(scratch + BM_LIST + j);
+                        place += (w.x > k) + (w.y > k);
+                    }
+                    __syncwarp();
+                    if (moved < width) scratch[BM_LIST + moved] = list;
+                    if (k > bar && place < width) scratch[BM_LIST + place] = k;
+                    __syncwarp();
+                    list = lane < width ? scratch[BM_LIST + lane] : 0;
+                    bar = scratch[BM_LIST + width - 1];
+                    __syncwarp();
                 }
+                if (lane == 0 && (uint32_t)(bar >> 32) > reach) atomicMax(const_cast<uint32_t*>(floor), (uint32_t)(bar >> 32));
             }
         }
         // lanes' maxima and sums -> the warp's
@@ -281,18 +317,36 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
         own.key[i] = r;
     }
     __syncthreads();
-    {   // each warp its run of items, then one warp the warps' winners
-        const int a = items * warp / BM_WARPS, e = items * (warp + 1) / BM_WARPS;
-        const uint64_t k = warp_select(own.key + (size_t)a * width, (e - a) * width, width, lane);
-        if (lane < width) best[warp * width + lane] = k;
+    {   // each warp the best of its run of items; then every winner counts the winners ahead of it
+        const int a = items * warp / BM_WARPS, e = items * (warp + 1) / BM_WARPS, count = (e - a) * width;
+        const uint64_t* mem = own.key + (size_t)a * width;
+        if (count <= 32) {
+            const uint64_t k = lane < count ? mem[lane] : 0;
+            int place = 0;
+#pragma unroll 4
+            for (int j = 0; j < count; ++j) place += mem[j] > k;
+            if (lane < width) best[warp * width + lane] = 0;
+            __syncwarp();
+            if (k != 0 && place < width) best[warp * width + place] = k;
+        } else {
+            const uint64_t k = warp_select(mem, count, width, lane);
+            if (lane < width) best[warp * width + lane] = k;
+        }
     }
     __syncthreads();
-    if (warp == 0) {
-        const uint64_t k = warp_select(best, BM_WARPS * width, width, lane);
-        if (lane < width) {
+    const int total = BM_WARPS * width;                             // at most one per thread
+    if (threadIdx.x < total) {
+        const uint64_t k = best[threadIdx.x];
+        int place = 0;
+#pragma unroll 4
+        for (int j = 0; j < total; j += 2) {
+            const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(best + j);
+            place += (w.x > k) + (w.y > k);
+        }
+        if (k != 0 && place < width) {
             const uint32_t at = ~(uint32_t)k;
             const int b = (int)(at / (uint32_t)V);
-            const int64_t t = at - (uint32_t)b * (uint32_t)V, o = entry * width + lane;
+            const int64_t t = at - (uint32_t)b * (uint32_t)V, o = entry * width + place;
             out_scores[o] = unordered((uint32_t)(k >> 32));
             parents[o] = b;
             tokens[o] = t;
