@@ -163,7 +163,7 @@ class FCSoftRows(torch.autograd.Function):
         ctx.shape = x.shape
         B = x.shape[0]
         x, kept = x.reshape(B, -1), None
-        if B and _keep_checkpoint(ctx):
+        if 0 < B <= 65535 * 128 and _keep_checkpoint(ctx):      # the fused kernel's grid
             xt, *kept = op("to_feature_major_ckpt")(x, ldb_for(B))
         else:
             xt = op("to_feature_major")(x, ldb_for(B))

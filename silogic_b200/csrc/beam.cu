@@ -531,6 +531,7 @@ extern "C" int slg_beam_reorder_rows(const void* in, int64_t row_bytes, const in
     };
     if (row_bytes % 16 == 0 && aligned16(in) && aligned16(out)) go(uint4());
     else if (row_bytes % 4 == 0 && aligned_to(in, 4) && aligned_to(out, 4)) go(uint32_t());
+    else if (row_bytes % 2 == 0 && aligned_to(in, 2) && aligned_to(out, 2)) go(uint16_t());
     else go(uint8_t());
     return check_launch("slg_beam_reorder_rows");
 }

@@ -375,3 +375,18 @@ def test_transpose_and_store_in_one_pass(B, F):
     wc, wb = IMPL["ckpt_store"](want[:, :B])
     eq = lambda a, b: torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))       # noqa: E731
     assert eq(out, want) and eq(bounds, wb) and torch.equal(codes[:, :ldb], wc[:, :ldb])
+
+
+@pytest.mark.parametrize("on", [False, True])
+def test_a_single_layer_traces_under_torch_compile(on):
+    torch.manual_seed(0)
+    layer = S.LogicLayer(40, 60, node="gate16", k=4, seed=0).to(dev)
+    f = torch.compile(layer, backend="aot_eager", fullgraph=True)
+    x = torch.rand(50, 40, device=dev, requires_grad=True)
+    gy = torch.randn(50, 60, device=dev)
+    wanted = [x] + list(layer.parameters())
+    with S.checkpoint8(on):
+        y0, y1 = layer(x), f(x)
+    assert torch.equal(y0, y1)
+    for a, b in zip(torch.autograd.grad(y1, wanted, gy), torch.autograd.grad(y0, wanted, gy)):
+        _close(a, b.double(), "compiled")
