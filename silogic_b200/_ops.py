@@ -327,6 +327,7 @@ def _(ids, g, V, scale, padding_idx):
 
 # --------------------------------------------------- 8-bit activation checkpoints
 CKPT_BLOCK = 128        # columns per (lo, step) pair (SLG_CKPT_BLOCK)
+_CKPT_BUILT = {}        # (K, node, arity) -> whether a backward kernel reads codes directly
 
 
 @_op("ckpt_store")
@@ -397,7 +398,10 @@ def fc_soft_bwd_ckpt(codes: Tensor, bounds: Tensor, ldb: int, cand: Tensor, conn
                      inv_tau: float, out_dim: int, wire_r: int, gy: Tensor,
                      need_gx: bool) -> Tuple[Tensor, Tensor, Tensor]:
     """:func:`fc_soft_bwd` at the activations that an 8-bit checkpoint stands for."""
-    if lib().slg_fc_soft_bwd_ckpt_built(K, node, arity):
+    built = _CKPT_BUILT.get((K, node, arity))
+    if built is None:
+        built = _CKPT_BUILT[K, node, arity] = bool(lib().slg_fc_soft_bwd_ckpt_built(K, node, arity))
+    if built:
         gy = gy.contiguous()
         gx = gy.new_zeros((codes.shape[0], ldb)) if need_gx else None
         gparams = torch.empty_like(params)

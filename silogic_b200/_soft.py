@@ -12,6 +12,7 @@ import torch
 from . import _hard
 from ._ops import op
 from ._lib import require_cuda
+from .connectomes import FixedConnectome, TopKConnectome
 
 
 NODE_ID = {"gate16": 0, "walsh": 1, "multilinear": 2, "hybrid": 3, "linear": 4}
@@ -63,31 +64,34 @@ class FromFeatureMajor(torch.autograd.Function):
 
 # --------------------------------------------------------------- FC layer
 def fc_supported(layer):
-    from .connectomes import FixedConnectome, TopKConnectome
-    if layer.node.kind not in NODE_ID and layer.node.kind != "polynomial":
+    return _fc_supported(layer, layer._conn, layer.node)
+
+
+def _fc_supported(layer, conn, node):
+    if node.kind not in NODE_ID and node.kind != "polynomial":
         return False
-    if not isinstance(layer._conn, (FixedConnectome, TopKConnectome)):
+    if not isinstance(conn, (FixedConnectome, TopKConnectome)):
         return False
-    if isinstance(layer._conn, TopKConnectome) and layer._conn.k > 16:
+    if isinstance(conn, TopKConnectome) and conn.k > 16:
         return False
-    if layer.node.kind == "walsh" and layer.node.gate_select == "gumbel" and layer.training:
+    if node.kind == "walsh" and node.gate_select == "gumbel" and layer.training:
         return False
     return 1 <= layer.arity <= 6
 
 
 def _fc_meta(layer, wire_r=0):
     """Static launch description of a LogicLayer's soft kernel."""
-    from .connectomes import FixedConnectome, TopKConnectome
-    if not fc_supported(layer):
+    connectome, node = layer._conn, layer.node      # a module's attributes are looked up slowly
+    if not _fc_supported(layer, connectome, node):
         raise NotImplementedError(
-            f"no soft kernel for node={layer.node.kind!r} connectome={type(layer._conn).__name__} "
+            f"no soft kernel for node={node.kind!r} connectome={type(connectome).__name__} "
             f"arity={layer.arity} in silogic_b200")
-    node = layer.node
     kind = node.kind
-    if isinstance(layer._conn, FixedConnectome):
-        cand, K, ste, conn = layer._conn.cand_i32, 1, 0, None
+    cand = connectome.cand_i32
+    if isinstance(connectome, FixedConnectome):
+        K, ste, conn = 1, 0, None
     else:
-        cand, K, ste, conn = layer._conn.cand_i32, layer._conn.k, int(layer._conn.ste), layer._conn.conn
+        K, ste, conn = connectome.k, int(connectome.ste), connectome.conn
     gate_hard = 0
     params = node.param
     if kind == "gate16" and layer.training:
@@ -182,14 +186,15 @@ def logic_layer_forward(layer, x):
     """``LogicLayer.forward`` on ``[B, in]``."""
     require_cuda(x)
     meta, params, conn = _fc_meta(layer)
-    meta["batch"] = x.shape[0]
+    B = meta["batch"] = x.shape[0]
+    if torch.compiler.is_compiling():       # one autograd Function inside another is not traced
+        return FromFeatureMajor.apply(FCSoft.apply(ToFeatureMajor.apply(x), params, conn, meta), B)
     return FCSoftRows.apply(x, params, conn, meta)
 
 
 def node_forward(node, x, idx):
     """``Node.forward`` on operands flattened to ``[B, out*arity]`` (identity wiring)."""
     from types import SimpleNamespace
-    from .connectomes import FixedConnectome
     conn = FixedConnectome.__new__(FixedConnectome)
     torch.nn.Module.__init__(conn)
     conn.cand_i32 = idx.unsqueeze(-1).contiguous()

@@ -54,7 +54,9 @@ def beam_step(logits, scores, finished=None, eos=None, width=None):
     x = logits if logits.dim() == 2 else logits.reshape(B * beams, V)
     if B and (x.stride(1) != 1 and V > 1 or x.stride(0) < V):
         x = x.contiguous()
-    scores = scores.detach().float().contiguous()
+    if scores.requires_grad or logits.requires_grad:      # a choice has no gradient
+        scores, x = scores.detach(), x.detach()
+    scores = scores.float().contiguous()
     out = scores.new_empty((B, width))
     parents, tokens = scores.new_empty((2, B, width), dtype=torch.int64).unbind(0)
     done = scores.new_empty((B, width), dtype=torch.bool) if eos is not None else None
@@ -79,7 +81,9 @@ def beam_reorder(state, parents, layout="rows", beams=None):
     B, width = parents.shape
     parents = parents.contiguous()
     st = stream_ptr(state.device)
-    state = state.detach().contiguous()
+    if state.requires_grad:
+        state = state.detach()
+    state = state.contiguous()
     if layout == "rows":
         if beams is None:
             beams = state.shape[0] // B if B else width

@@ -50,7 +50,8 @@ def checkpoint8_store(x):
     if x.dim() == 0:
         raise ValueError("checkpoint8_store: x must have at least one dimension")
     require_cuda(x)
-    x = x.detach()
+    if x.requires_grad:
+        x = x.detach()
     if x.numel() == 0:
         rows, cols = 0, x.shape[-1]
         return Checkpoint8(torch.empty((rows, cols), dtype=torch.uint8, device=x.device),
