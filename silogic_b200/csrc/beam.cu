@@ -103,7 +103,7 @@ __host__ __device__ inline int beam_parts(int cs, int beams, int units) {
     const int p = cs * BM_WARPS / beams;
     return p < 1 ? 1 : p < units ? p : units;
 }
-// at most 38,144 bytes (8 CTAs, 32 beams, width 32) beside the warps' 8,448 of scratch
+// at most 38,144 bytes (8 CTAs, 32 beams, width 32) beside 8,672 of fixed size
 constexpr int BM_LIST = 34;             // candidates and a 0 before a warp's list in its scratch
 constexpr int BM_SCRATCH = BM_LIST + 32;
 static inline size_t beam_smem(int items, int beams, int width) {
@@ -150,15 +150,22 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
     float* beam_m = own.s + items;                                  // [beams] maximum, log of the sum
     float* beam_l = beam_m + beams;
 
+    __shared__ float own_score[BM_MAX];         // the entry's beams, read here for the join
+    __shared__ uint8_t own_done[BM_MAX];
+
     uint64_t* scratch = scratches[warp];
     if (threadIdx.x < BM_WARPS) floors[threadIdx.x] = 0;
+    if (threadIdx.x < beams) {
+        own_score[threadIdx.x] = scores[entry * beams + threadIdx.x];
+        own_done[threadIdx.x] = finished && finished[entry * beams + threadIdx.x];
+    }
     __syncthreads();
     auto started = cluster.barrier_arrive();                        // the first CTA's memory is there
     bool waited = false;
     for (int item = rank * BM_WARPS + warp; item < items; item += cs * BM_WARPS) {
         const int b = item / parts, part = item - b * parts;
         const int64_t row_at = entry * beams + b;
-        const bool done = finished && finished[row_at];
+        const bool done = own_done[b];
         // the warps of a beam share its floor (with one part per beam a warp has its own)
         volatile uint32_t* floor = &floors[parts > 1 ? b - rank * BM_WARPS / parts : warp];
         if (parts == 1) *floor = 0;
@@ -308,9 +315,8 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
         const uint64_t k = own.key[i];
         uint64_t r = 0;
         if (k != 0) {
-            const float S = scores[entry * beams + b], x = unordered((uint32_t)(k >> 32));
-            const bool done = finished && finished[entry * beams + b];
-            float v = done ? x + S : beam_m[b] > -CUDART_INF_F ? (x - beam_m[b]) - beam_l[b] + S : -CUDART_INF_F;
+            const float S = own_score[b], x = unordered((uint32_t)(k >> 32));
+            float v = own_done[b] ? x + S : beam_m[b] > -CUDART_INF_F ? (x - beam_m[b]) - beam_l[b] + S : -CUDART_INF_F;
             if (v != v) v = -CUDART_INF_F;
             r = cand_key(v, (uint32_t)b * (uint32_t)V + ~(uint32_t)k);
         }
@@ -350,7 +356,7 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
             out_scores[o] = unordered((uint32_t)(k >> 32));
             parents[o] = b;
             tokens[o] = t;
-            if (out_finished) out_finished[o] = (finished && finished[entry * beams + b]) || t == eos;
+            if (out_finished) out_finished[o] = own_done[b] || t == eos;
         }
     }
 }
@@ -421,14 +427,13 @@ reorder_features_kernel(const float* __restrict__ in, int64_t F, int64_t ldi, in
 // four words, which are loaded first.
 constexpr int RP_THREADS = 256;
 constexpr int RP_WORDS = 32;
-constexpr int RP_PER = 2;               // words per thread
 template <bool FOUR>
 __global__ void __launch_bounds__(RP_THREADS)
 reorder_packed_kernel(const uint32_t* __restrict__ in, int64_t F, int64_t ldi, int64_t n,
                       const int64_t* __restrict__ parents, int beams, int width, uint32_t* __restrict__ out,
                       int64_t ldo) {
     __shared__ int64_t word_of[RP_WORDS];       // first source word of an output word
-    __shared__ uint16_t from[RP_WORDS][34];     // bit's source: 32 (word - first) + bit, 0xffff: none
+    __shared__ __align__(4) uint16_t from[RP_WORDS][34];     // bit's source: 32 (word - first) + bit, 0xffff: none
     const int64_t w0 = (int64_t)blockIdx.y * RP_WORDS;
     const int words = (int)min((int64_t)RP_WORDS, ldo - w0);
     for (int i = threadIdx.x; i < words * 32; i += RP_THREADS) {
@@ -441,10 +446,8 @@ reorder_packed_kernel(const uint32_t* __restrict__ in, int64_t F, int64_t ldi, i
     }
     __syncthreads();
     const int64_t total = F * words;
-#pragma unroll
-    for (int u = 0; u < RP_PER; ++u) {
-        const int64_t t = ((int64_t)blockIdx.x * RP_PER + u) * RP_THREADS + threadIdx.x;
-        if (t >= total) continue;
+    const int64_t t = (int64_t)blockIdx.x * RP_THREADS + threadIdx.x;
+    if (t < total) {
         const int64_t f = total < (1ll << 32) ? (int64_t)((uint32_t)t / (uint32_t)words) : t / words;
         const int w = (int)(t - f * words);
         const int64_t first = word_of[w];
@@ -458,10 +461,15 @@ reorder_packed_kernel(const uint32_t* __restrict__ in, int64_t F, int64_t ldi, i
 #pragma unroll
             for (int q = 0; q < 4; ++q) x[q] = first + q < ldi ? __ldg(src + q) : 0u;
 #pragma unroll 8
-            for (int j = 0; j < 32; ++j) {
-                const uint32_t s = from[w][j];
-                const uint32_t lo = s & 32u ? x[1] : x[0], hi = s & 32u ? x[3] : x[2];
-                if (s != 0xffffu) bits |= ((s & 64u ? hi : lo) >> (s & 31u) & 1u) << j;
+            for (int j = 0; j < 32; j += 2) {
+                const uint32_t two = *reinterpret_cast<const uint32_t*>(&from[w][j]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t s = h ? two >> 16 : two & 0xffffu;
+                    const uint32_t lo = s & 32u ? x[1] : x[0], hi = s & 32u ? x[3] : x[2];
+                    const uint32_t bit = (s & 64u ? hi : lo) >> (s & 31u) & 1u;
+                    bits |= (s == 0xffffu ? 0u : bit) << (j + h);
+                }
             }
         } else {
 #pragma unroll 8
@@ -557,7 +565,7 @@ extern "C" int slg_beam_reorder_packed(const uint64_t* in, int64_t F, int64_t ld
         return set_error(SLG_ERR_ARG, "slg_beam_reorder_packed: bad sizes");
     const int64_t per_row = std::min<int64_t>(2 * ldo, RP_WORDS), tiles = cdiv(2 * ldo, RP_WORDS);
     if (tiles > 65535) return set_error(SLG_ERR_ARG, "slg_beam_reorder_packed: batch too large");
-    const dim3 grid((unsigned)cdiv(F * per_row, RP_THREADS * RP_PER), (unsigned)tiles);
+    const dim3 grid((unsigned)cdiv(F * per_row, RP_THREADS), (unsigned)tiles);
     auto go = [&](auto kernel) {
         kernel<<<grid, RP_THREADS, 0, as_stream(stream)>>>(reinterpret_cast<const uint32_t*>(in), F, 2 * ldi, B * width,
                                                            parents, beams, width, reinterpret_cast<uint32_t*>(out), 2 * ldo);
