@@ -510,7 +510,10 @@ extern "C" int slg_beam_step(const void* logits, int32_t dtype, int64_t B, int32
         e = beam_step_launch<T>((const T*)logits, B, beams, V, ldx, scores, finished, eos, width, out_scores, parents,
                                 tokens, out_finished, as_stream(stream));
     });
-    if (e != cudaSuccess) return set_error(SLG_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
+    if (e != cudaSuccess) {
+        cudaGetLastError();             // reported here: the next call starts clean
+        return set_error(SLG_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
+    }
     return check_launch(name);
 }
 
