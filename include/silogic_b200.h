@@ -394,7 +394,7 @@ int slg_to_feature_major_ckpt(const float* x, int64_t B, int64_t F, float* out, 
 /* slg_fc_soft_bwd with the layer's input read from an 8-bit checkpoint of its
  * feature-major activations: codes [in_dim, ldc], bounds [in_dim,
  * ceil(ldb / SLG_CKPT_BLOCK), 2]; the other arguments and the workspace are those of
- * slg_fc_soft_bwd.  Built for the (K, node, arity) that _built() answers with 1; for the
+ * slg_fc_soft_bwd, except that gx is written (zeroed here), not added to.  Built for the (K, node, arity) that _built() answers with 1; for the
  * others restore the activations (slg_ckpt_load) and call slg_fc_soft_bwd. */
 int32_t slg_fc_soft_bwd_ckpt_built(int32_t K, int32_t node, int32_t arity);
 int slg_fc_soft_bwd_ckpt(const uint8_t* codes, int64_t ldc, const float* bounds, int64_t in_dim,

@@ -403,7 +403,7 @@ def fc_soft_bwd_ckpt(codes: Tensor, bounds: Tensor, ldb: int, cand: Tensor, conn
         built = _CKPT_BUILT[K, node, arity] = bool(lib().slg_fc_soft_bwd_ckpt_built(K, node, arity))
     if built:
         gy = gy.contiguous()
-        gx = gy.new_zeros((codes.shape[0], ldb)) if need_gx else None
+        gx = gy.new_empty((codes.shape[0], ldb)) if need_gx else None
         gparams = torch.empty_like(params)
         gconn = torch.empty_like(conn) if conn is not None else None
         nbytes = lib().slg_fc_soft_workspace_bytes(ldb, K, node, arity, out_dim)

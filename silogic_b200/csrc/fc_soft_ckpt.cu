@@ -272,12 +272,16 @@ extern "C" int slg_fc_soft_bwd_ckpt(const uint8_t* codes, int64_t ldc, const flo
     if (workspace_bytes < need)
         return set_error(SLG_ERR_WORKSPACE, "%s: workspace %lld < %lld bytes", name, (long long)workspace_bytes,
                          (long long)need);
-    if (out_dim == 0) return SLG_OK;
     const FcArgs A{nullptr, in_dim, ldb, cand, conn, K, conn_ste, params, gate_hard, inv_tau, out_dim, wire_r};
     const uint32_t* c = reinterpret_cast<const uint32_t*>(codes);
     const float2* b = reinterpret_cast<const float2*>(bounds);
     float* ws = static_cast<float*>(workspace);
     cudaStream_t s = as_stream(stream);
+    if (gx) {
+        const cudaError_t err = cudaMemsetAsync(gx, 0, (size_t)in_dim * (size_t)ldb * 4, s);
+        if (err != cudaSuccess) return set_error(SLG_ERR_CUDA, "%s: %s", name, cudaGetErrorString(err));
+    }
+    if (out_dim == 0) return SLG_OK;
     auto go = [&](auto node_tag) {
         constexpr int NODE = decltype(node_tag)::value;
         if (K == 1) launch_ckpt<NODE, 1>(A, c, ldc / 4, b, gy, gx, ws, gconn, gparams, s);

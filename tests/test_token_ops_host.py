@@ -117,7 +117,7 @@ def test_checkpoint_backward_refuses_bad_arguments(L):
         assert call(**{name: 0}) == 1, name
     assert call(gy=264) == 2 and call(gx=264) == 2 and call(codes=258) == 2 and call(bounds=260) == 2
     assert call(size=need - 1) == 5
-    assert call(O=0) == 0
+    assert call(O=0, gx=0) == 0
     for K, node, ar, want in ((8, 0, 2, 1), (1, 3, 2, 1), (9, 0, 2, 0), (4, 1, 3, 0), (4, 4, 2, 0), (4, 5, 2, 0), (0, 1, 2, 0)):
         assert L.slg_fc_soft_bwd_ckpt_built(K, node, ar) == want
 
