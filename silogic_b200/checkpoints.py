@@ -9,6 +9,8 @@ step, 1/510 of the block's range).  Binary inputs are kept exactly.
     with silogic_b200.checkpoint8():
         loss = criterion(model(x), y)
     loss.backward()
+
+``train_model`` and ``GraphedTrainStep`` called inside the context train that way too.
 """
 import contextlib
 

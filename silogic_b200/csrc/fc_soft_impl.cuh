@@ -82,7 +82,7 @@ fc_soft_fwd_kernel(const float4* __restrict__ x, int64_t nv, const int32_t* __re
             wr[j * KT + k] = on ? S.w[j * K + k] : 0.0f;
         }
     // Zero weights (one-hot selection) skip their loads; a node that has none takes the loop
-    // without the tests, which cost a tenth of the time (10,000 Top-8 Walsh nodes x 4,096
+    // without the tests, which cost a fifth of the time (10,000 Top-8 Walsh nodes x 4,096
     // samples: 285 -> 226 us).
     bool dense = true;
 #pragma unroll
