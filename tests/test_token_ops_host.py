@@ -81,6 +81,12 @@ def test_c_entry_points_refuse_bad_arguments(L):
     assert store(rows=-1) == 1 and store(ldx=9) == 1 and store(ldc=8) == 1 and store(ldc=11) == 2
     assert store(dt=9) == 3 and store(codes=0) == 1 and store(x=0) == 1 and store(codes=258) == 2 and store(bounds=260) == 2
     assert store(rows=0, codes=0, bounds=0, x=0) == 0
+    both = lambda x=256, B=130, F=7, out=256, ldb=132, codes=256, ldc=144, bounds=256: L.slg_to_feature_major_ckpt(  # noqa: E731
+        _p(x), B, F, _p(out), ldb, _p(codes), ldc, _p(bounds), _p(0))
+    assert both(B=0) == 1 and both(F=-1) == 1 and both(ldb=129) == 1 and both(ldc=131) == 1
+    assert both(ldb=260, ldc=272) == 1 and b"last block" in L.slg_last_error()
+    assert both(x=0) == 1 and both(out=0) == 1 and both(codes=0) == 1 and both(bounds=0) == 1 and both(bounds=260) == 2
+    assert both(F=0, x=0) == 0
     load = lambda x=256, rows=4, cols=10, ldx=10, codes=256, ldc=12, bounds=256, dt=0: L.slg_ckpt_load(    # noqa: E731
         _p(codes), ldc, _p(bounds), rows, cols, _p(x), dt, ldx, _p(0))
     assert load(cols=-1) == 1 and load(ldc=11) == 2 and load(dt=-1) == 3 and load(x=0) == 1
