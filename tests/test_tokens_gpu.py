@@ -59,7 +59,7 @@ def test_lookup_and_gradient_match_64_bits(V, D, N, dtype):
     _check_grad(gw, ids, gy, V, scale)
 
 
-@pytest.mark.parametrize("N", [0, 1, 31, 4096, 4097, 9000, 300000])
+@pytest.mark.parametrize("N", [0, 1, 31, 1024, 1025, 4096, 4097, 8192, 8193, 9000, 300000])
 def test_gradient_of_one_hot_token_and_empty_batch(N):
     """Every token the same: one row takes the whole sum, the others are zero."""
     ids, w, gy = _case(37, 20, N, torch.float32, ids=torch.full((N,), 5))
