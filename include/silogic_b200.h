@@ -421,8 +421,9 @@ int slg_beam_step(const void* logits, int32_t dtype, int64_t B, int32_t beams, i
 /* Decoder state after a step: sample r = e * width + n of `out` is sample
  * e * beams + parents[e, n] of `in` (a parent outside [0, beams) reads beam 0).
  * rows: [samples, row_bytes] of any type; features: feature-major fp32 [F, ld]; packed:
- * bit-packed [F, ld] uint64.  Padding columns and bits are written 0.  `out` must not
- * overlap `in`. */
+ * bit-packed [F, ld] uint64 (SLG_ERR_UNSUPPORTED from about 2^27 beams an entry on).
+ * Padding columns and bits are written 0; beams and width are not limited to
+ * SLG_BEAM_MAX.  `out` must not overlap `in`. */
 int slg_beam_reorder_rows(const void* in, int64_t row_bytes, const int64_t* parents, int64_t B,
                           int32_t beams, int32_t width, void* out, void* stream);
 int slg_beam_reorder_features(const float* in, int64_t F, int64_t ldi, const int64_t* parents,

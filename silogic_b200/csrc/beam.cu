@@ -423,25 +423,34 @@ reorder_features_kernel(const float* __restrict__ in, int64_t F, int64_t ldi, in
 // The same on bits.  A thread builds one 32-bit word of a row bit by bit; a CTA's threads
 // walk (row, word) of 32 word columns, row by row, so stores are whole lines (a warp that
 // built one word by ballot stored 4 bytes at a time: 10 us on 10,000 x 512).  The sources of the
-// 1,024 samples are worked out once per CTA.  With width >= beams a word's sources lie in
-// four words, which are loaded first.
+// 1,024 samples are worked out once per CTA.  FOUR: a word's sources lie in four words, which are
+// loaded first (sources_in_four below); otherwise every bit loads its word.
 constexpr int RP_THREADS = 256;
 constexpr int RP_WORDS = 32;
+constexpr uint32_t RP_NONE = 0xffffffffu;
+
+// A word's first sample is at most width - 1 into its entry, so its last one's entry begins at
+// most (width + 30) / width entries after the first's, and that many times `beams` samples; the
+// first source word begins at most 31 samples before its entry's first.
+inline int64_t last_source_offset(int64_t beams, int64_t width) { return 31 + ((width + 30) / width) * beams + beams - 1; }
+inline bool sources_in_four(int64_t beams, int64_t width) { return last_source_offset(beams, width) < 128; }
+
 template <bool FOUR>
 __global__ void __launch_bounds__(RP_THREADS)
 reorder_packed_kernel(const uint32_t* __restrict__ in, int64_t F, int64_t ldi, int64_t n,
                       const int64_t* __restrict__ parents, int beams, int width, uint32_t* __restrict__ out,
                       int64_t ldo) {
     __shared__ int64_t word_of[RP_WORDS];       // first source word of an output word
-    __shared__ __align__(4) uint16_t from[RP_WORDS][34];     // bit's source: 32 (word - first) + bit, 0xffff: none
+    // bit's source: 32 (word - first) + bit; FOUR reads two at a time, and needs 7 bits
+    using From = typename std::conditional<FOUR, uint16_t, uint32_t>::type;
+    __shared__ __align__(4) From from[RP_WORDS][FOUR ? 34 : 33];
     const int64_t w0 = (int64_t)blockIdx.y * RP_WORDS;
     const int words = (int)min((int64_t)RP_WORDS, ldo - w0);
     for (int i = threadIdx.x; i < words * 32; i += RP_THREADS) {
-        // an output word's 32 samples span at most 31 / width + 2 entries of at most 32 beams
         const int64_t r0 = (w0 + i / 32) * 32, r = r0 + i % 32;
         const int64_t first = ((int64_t)((uint32_t)r0 / (uint32_t)width) * beams) >> 5;
         from[i / 32][i % 32] =
-            r < n ? (uint16_t)(beam_source(parents, (uint32_t)r, beams, width) - first * 32) : (uint16_t)0xffff;
+            r < n ? (From)(beam_source(parents, (uint32_t)r, beams, width) - first * 32) : (From)RP_NONE;
         if (i % 32 == 0) word_of[i / 32] = first;
     }
     __syncthreads();
@@ -454,9 +463,6 @@ reorder_packed_kernel(const uint32_t* __restrict__ in, int64_t F, int64_t ldi, i
         const uint32_t* src = in + f * ldi + first;
         uint32_t bits = 0;
         if constexpr (FOUR) {
-            // the word's first sample is at most width - 1 into its entry, so its last one's
-            // entry begins at most (width + 30) beams / width <= 62 samples after the first's:
-            // offsets stay below 31 + 62 + 32 < 128
             uint32_t x[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) x[q] = first + q < ldi ? __ldg(src + q) : 0u;
@@ -475,7 +481,7 @@ reorder_packed_kernel(const uint32_t* __restrict__ in, int64_t F, int64_t ldi, i
 #pragma unroll 8
             for (int j = 0; j < 32; ++j) {
                 const uint32_t s = from[w][j];
-                if (s != 0xffffu) bits |= (__ldg(src + (s >> 5)) >> (s & 31u) & 1u) << j;
+                if (s != RP_NONE) bits |= (__ldg(src + (s >> 5)) >> (s & 31u) & 1u) << j;
             }
         }
         out[f * ldo + w0 + w] = bits;
@@ -568,12 +574,14 @@ extern "C" int slg_beam_reorder_packed(const uint64_t* in, int64_t F, int64_t ld
         return set_error(SLG_ERR_ARG, "slg_beam_reorder_packed: bad sizes");
     const int64_t per_row = std::min<int64_t>(2 * ldo, RP_WORDS), tiles = cdiv(2 * ldo, RP_WORDS);
     if (tiles > 65535) return set_error(SLG_ERR_ARG, "slg_beam_reorder_packed: batch too large");
+    if (last_source_offset(beams, width) >= (int64_t)RP_NONE)
+        return set_error(SLG_ERR_UNSUPPORTED, "slg_beam_reorder_packed: %d beams per entry", beams);
     const dim3 grid((unsigned)cdiv(F * per_row, RP_THREADS), (unsigned)tiles);
     auto go = [&](auto kernel) {
         kernel<<<grid, RP_THREADS, 0, as_stream(stream)>>>(reinterpret_cast<const uint32_t*>(in), F, 2 * ldi, B * width,
                                                            parents, beams, width, reinterpret_cast<uint32_t*>(out), 2 * ldo);
     };
-    if (width >= beams) go(reorder_packed_kernel<true>);
+    if (sources_in_four(beams, width)) go(reorder_packed_kernel<true>);
     else go(reorder_packed_kernel<false>);
     return check_launch("slg_beam_reorder_packed");
 }

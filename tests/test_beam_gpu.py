@@ -305,3 +305,18 @@ def test_example_trains_and_decodes():
         ids = logits.argmax(1)
         assert torch.equal(ids, tokens[:, 0, t])
         logits, h = step(ids, h)
+
+
+@pytest.mark.parametrize("B,k,w", [(3, 48, 48), (3, 49, 49), (2, 51, 51), (3, 64, 64), (2, 100, 100), (1, 200, 200),
+                                   (2, 3, 120), (2, 40, 90), (1, 2100, 7), (2, 5000, 3), (1, 4096, 4096), (9, 33, 5)])
+def test_reorder_packed_with_more_beams_than_a_step_has(B, k, w):
+    """beam_reorder takes any number of beams: a word's sources then lie in more than four words,
+    or further than 16 bits apart."""
+    g = torch.Generator().manual_seed(k + w)
+    parents = torch.randint(0, k, (B, w), generator=g).to(dev)
+    parents[:, -1], parents[:, 0] = 0, k - 1
+    bits = (torch.rand(B * k, 37, generator=g) > 0.5).to(torch.uint8).to(dev)
+    got = S.beam_reorder(_hard.pack(bits), parents, layout="packed", beams=k)
+    want = bits[_src(parents, k)].contiguous()
+    assert torch.equal(_hard.unpack(got, B * w), want)
+    assert torch.equal(got, _hard.pack(want, ldw=got.shape[1]))

@@ -136,3 +136,11 @@ def test_packed_reorder_sources_lie_in_four_words(beams):
             first = (word * 32 // width * beams) >> 5
             last = ((word * 32 + 31) // width) * beams + beams - 1
             assert last - 32 * first < 128
+
+
+def test_packed_reorder_refuses_offsets_past_32_bits(L):
+    """A word of 32 samples of one-beam results spans 32 entries of the state's beams."""
+    beams = 1 << 28
+    packed = lambda width, ldi: L.slg_beam_reorder_packed(_p(256), 3, ldi, _p(256), 1, beams, width, _p(512), 1, _p(0))   # noqa: E731
+    assert packed(1, beams // 64) == 3 and b"beams per entry" in L.slg_last_error()
+    assert packed(1, beams // 64 - 1) == 1                                 # rows too short
