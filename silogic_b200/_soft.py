@@ -7,6 +7,8 @@ Every Function's backward is a CUDA kernel too; parameter-side transforms
 (connection softmax, gate_probs @ basis, sigmoid of LUT logits) are fused into
 the layer kernels.
 """
+import threading
+
 import torch
 
 from . import _hard
@@ -22,13 +24,25 @@ def ldb_for(B):
     return max(4, (int(B) + 3) // 4 * 4)
 
 
-#: set by :func:`silogic_b200.checkpoint8`: layers keep their input for the backward pass
-#: as 8-bit codes instead of fp32
-CHECKPOINT8 = False
+#: ``_switch.on``, set by :func:`silogic_b200.checkpoint8`: this thread's layers keep their
+#: input for the backward pass as 8-bit codes instead of fp32.  A plain attribute of a
+#: ``threading.local``: torch.compile guards on its value in the calling thread (it cannot
+#: trace a ``ContextVar``, and does not guard on a class attribute of a subclass).
+_switch = threading.local()
+
+
+def checkpointing():
+    return getattr(_switch, "on", False)
+
+
+def __getattr__(name):
+    if name == "CHECKPOINT8":
+        return checkpointing()
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 def _keep_checkpoint(ctx):
-    return CHECKPOINT8 and any(ctx.needs_input_grad[:3])
+    return checkpointing() and any(ctx.needs_input_grad[:3])
 
 
 def _store(xt, meta):

@@ -64,11 +64,16 @@ def checkpoint8_store(x):
 
 @contextlib.contextmanager
 def checkpoint8(enabled=True):
-    """Layers run inside keep their inputs for the backward pass as 8-bit codes (the setting
-    is process-wide; ``enabled=False`` switches it off inside)."""
-    before = _soft.CHECKPOINT8
-    _soft.CHECKPOINT8 = bool(enabled)
+    """Layers run inside keep their inputs for the backward pass as 8-bit codes
+    (``enabled=False`` switches it off inside).  The setting is the calling thread's: other
+    threads are not affected, and a thread started inside begins with it off.  The innermost
+    context that is still open decides."""
+    mine = [bool(enabled)]          # an object of its own: contexts may end in any order
+    opened = _soft._switch.__dict__.setdefault("opened", [])
+    opened.append(mine)
+    _soft._switch.on = mine[0]
     try:
         yield
     finally:
-        _soft.CHECKPOINT8 = before
+        opened[:] = [c for c in opened if c is not mine]
+        _soft._switch.on = opened[-1][0] if opened else False

@@ -144,3 +144,56 @@ def test_packed_reorder_refuses_offsets_past_32_bits(L):
     packed = lambda width, ldi: L.slg_beam_reorder_packed(_p(256), 3, ldi, _p(256), 1, beams, width, _p(512), 1, _p(0))   # noqa: E731
     assert packed(1, beams // 64) == 3 and b"beams per entry" in L.slg_last_error()
     assert packed(1, beams // 64 - 1) == 1                                 # rows too short
+
+
+def test_checkpoint8_belongs_to_the_thread_that_sets_it():
+    """Two threads whose contexts overlap: neither sees nor leaves the other's setting."""
+    import threading
+    from silogic_b200 import _soft
+    inside, left = threading.Event(), threading.Event()
+    seen = {}
+
+    def first():
+        with S.checkpoint8():
+            inside.set()
+            assert left.wait(10)
+            seen["first, inside"] = _soft.CHECKPOINT8
+        seen["first, after"] = _soft.CHECKPOINT8
+    t = threading.Thread(target=first)
+    t.start()
+    assert inside.wait(10)
+    seen["other, before"] = _soft.CHECKPOINT8
+    with S.checkpoint8(False):
+        seen["other, off"] = _soft.CHECKPOINT8
+    with S.checkpoint8():
+        left.set()
+        t.join()
+        seen["other, inside"] = _soft.CHECKPOINT8
+    seen["other, after"] = _soft.CHECKPOINT8
+    assert seen == {"first, inside": True, "first, after": False, "other, before": False, "other, off": False,
+                    "other, inside": True, "other, after": False}
+
+
+def test_checkpoint8_contexts_of_one_thread_may_end_in_any_order():
+    """Generators and coroutines interleave contexts in one thread."""
+    from silogic_b200 import _soft
+    a, b = S.checkpoint8(), S.checkpoint8()
+    a.__enter__()
+    b.__enter__()
+    a.__exit__(None, None, None)
+    assert _soft.CHECKPOINT8 is True
+    b.__exit__(None, None, None)
+    assert _soft.CHECKPOINT8 is False
+
+
+def test_checkpoint8_is_read_again_by_a_traced_function():
+    """torch.compile guards on the thread's setting: a function traced outside is traced again inside."""
+    from silogic_b200 import _soft
+    f = torch.compile(lambda x: x * 2 if _soft.checkpointing() else x + 1, backend="eager", fullgraph=True)
+    x = torch.full((2,), 5.0)
+    assert f(x)[0] == 6
+    with S.checkpoint8():
+        assert f(x)[0] == 10
+        with S.checkpoint8(False):
+            assert f(x)[0] == 6
+    assert f(x)[0] == 6
