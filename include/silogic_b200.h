@@ -408,8 +408,9 @@ int slg_fc_soft_bwd_ckpt(const uint8_t* codes, int64_t ldc, const float* bounds,
  * (sums of log probabilities so far; -inf for a beam that is not in use).  Candidate
  * (b, v) has (x - max_b) - log(sum exp(x - max_b)) + scores[b]; a beam with finished[b]
  * != 0 has the one candidate (b, eos) at scores[b].  The `width` best of each entry come
- * out in order, equal values by the lowest b * V + v: their values, beams (parents), tokens and,
- * when out_finished is given, finished[parent] || token == eos.  NaN logits count as
+ * out in order, equal values (as rounded to 32 bits; different logits can tie) by the lowest
+ * b * V + v: their values, beams (parents), tokens and, when out_finished is given,
+ * finished[parent] || token == eos.  NaN logits count as
  * masked (-inf), +inf as the largest finite value; masked candidates (value -inf) come
  * last.  beams, width <= SLG_BEAM_MAX, V < 2^27; finished and out_finished may be NULL. */
 #define SLG_BEAM_MAX 32

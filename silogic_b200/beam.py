@@ -22,9 +22,10 @@ def beam_step(logits, scores, finished=None, eos=None, width=None):
     ``logits`` ``[B, beams, V]`` or ``[B * beams, V]`` (float32, bfloat16 or float16; class
     counts / tau of a circuit, or soft logits), ``scores`` ``[B, beams]`` = each beam's sum of log
     probabilities (-inf: not in use).  A candidate's score is
-    ``log_softmax(logits)[b, v] + scores[b]`` in 32 bits; equal scores go to the lowest beam,
-    then the lowest token.  A beam with ``finished[b]`` goes on with ``eos`` alone, at its score.
-    Masked logits (-inf or NaN) are chosen only when nothing else is left, with score -inf."""
+    ``log_softmax(logits)[b, v] + scores[b]`` in 32 bits; scores that are equal there (of
+    different logits too) go to the lowest beam, then the lowest token.  A beam with ``finished[b]`` goes on with ``eos`` alone, at its score.
+    Masked logits (-inf or NaN) and all candidates of a beam at -inf score -inf: they are
+    chosen only when nothing else is left, by beam and token too."""
     if scores.dim() != 2:
         raise ValueError(f"beam_step: scores must be [B, beams], got {tuple(scores.shape)}")
     B, beams = scores.shape

@@ -4,8 +4,8 @@
 //   l[b, v] = (x[b, v] - m_b) - log sum_u exp(x[b, u] - m_b) + S_b,    m_b = max_u x[b, u]
 // and the `width` largest l of an entry's beams, equal values by the lowest b V + v.  A
 // finished beam has the one candidate (b, eos) at its own score.  Masked logits (-inf, or
-// NaN) are never chosen while another candidate is left; +inf counts as the largest finite
-// value.  (x - m) - log s keeps rows apart whose logits are huge or at the type's lowest value.
+// NaN) and what else scores -inf come last; +inf counts as the largest finite value.  Values
+// are compared as they are rounded to 32 bits, so different logits can tie.  (x - m) - log s keeps rows apart whose logits are huge or at the type's lowest value.
 #include <cooperative_groups.h>
 #include <utility>
 
@@ -68,6 +68,15 @@ __device__ __forceinline__ uint64_t warp_max(uint64_t k) {
     return ((uint64_t)hi << 32) | lo;
 }
 
+// A candidate's score, from the beam's maximum m, logarithm l of its sum and score S.  Every
+// operation is monotone in x, so a beam's candidates in the order of their logits are in the
+// order of their scores -- but different logits can have the same score.
+__device__ __forceinline__ float beam_score(float x, float m, float l, float S) {
+    const float v = m > -CUDART_INF_F ? (x - m) - l + S : -CUDART_INF_F;
+    return v == v ? v : -CUDART_INF_F;
+}
+__device__ __forceinline__ float finished_score(bool is_eos, float S) { return is_eos && S == S ? S : -CUDART_INF_F; }
+
 // The n largest keys of mem[0 .. count), keys being distinct; lane i returns the i-th
 // (0: there is none).
 __device__ __forceinline__ uint64_t warp_select(const uint64_t* mem, int count, int n, int lane) {
@@ -91,23 +100,28 @@ __device__ __forceinline__ uint64_t warp_select(const uint64_t* mem, int count, 
 // largest logits (lane i: the i-th): a unit is only searched while one of its lanes' maxima
 // beats the list's last, so later units cost little more than their loads.  It leaves (max,
 // sum, list) in the first CTA's shared memory; that CTA joins maxima and sums per beam,
-// turns lists into scores, and selects.  Which lane sums which logits depends on their place in
+// turns lists into scores, and selects.  A list goes by logits, ties by token: a logit that it
+// lacks can have the score of the last chosen candidate and a lower index, so warps also keep the
+// largest logit that is in no list, and where its score reaches the last chosen one's the
+// candidates of that score are looked for in order (choose_equal).  Keeping it costs 25.9 -> 27.1 us
+// on 64 x 8 x 32,000 fp32 and 7.3 -> 7.9 on 1 x 4 x 2,000.  Which lane sums which logits depends on their place in
 // the row alone: beams with the same logits get the same normaliser, and tie.
 struct BeamSlots {
     uint64_t* key;          // [items][width] (ordered logit, ~token); then (ordered score, ~index)
     float* m;               // [items]
     float* s;               // [items]
+    uint32_t* out;          // [items] largest ordered logit that the list lacks, 0: none
 };
 
 __host__ __device__ inline int beam_parts(int cs, int beams, int units) {
     const int p = cs * BM_WARPS / beams;
     return p < 1 ? 1 : p < units ? p : units;
 }
-// at most 38,144 bytes (8 CTAs, 32 beams, width 32) beside 8,672 of fixed size
+// at most 38,784 bytes (8 CTAs, 32 beams, width 32) beside 8,756 of fixed size
 constexpr int BM_LIST = 34;             // candidates and a 0 before a warp's list in its scratch
 constexpr int BM_SCRATCH = BM_LIST + 32;
 static inline size_t beam_smem(int items, int beams, int width) {
-    return (size_t)(items * width + (items * width & 1)) * 8 + (size_t)BM_WARPS * width * 8 + (size_t)items * 8 + beams * 8;
+    return (size_t)(items * width + (items * width & 1)) * 8 + (size_t)BM_WARPS * width * 8 + (size_t)items * 12 + beams * 12;
 }
 
 // logits [at, at + E) of a row of V, masked past its end
@@ -124,6 +138,60 @@ __device__ __forceinline__ void load_logits(const T* __restrict__ row, bool alig
             const bool on = at + j < V;
             x[j] = on ? to_f32(row[at + j]) : -CUDART_INF_F;
             valid |= (on ? 1u : 0u) << (bit + j);
+        }
+    }
+}
+
+// Places `found` and up of the result: the candidates whose score is `last`, lowest index first.
+// One CTA reads the entry's logits again, 4,096 at a time, until the places are filled.  For ties
+// at the end of the result alone, which are short of lists (random fp32 logits: below one call in
+// a thousand) or found within the first tokens (scores all -inf, constant logits).
+constexpr int BM_AGAIN = 8;
+template <typename T>
+__device__ __noinline__ void choose_equal(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams, int64_t entry,
+                                          const float* score, const uint8_t* done, const float* m, const float* l,
+                                          int32_t eos, int width, float last, int found, int* sums,
+                                          float* __restrict__ out_scores, int64_t* __restrict__ parents,
+                                          int64_t* __restrict__ tokens, uint8_t* __restrict__ out_finished) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int b = 0; b < beams && found < width; ++b) {
+        const float S = score[b];
+        if ((done[b] ? finished_score(true, S) : beam_score(m[b], m[b], l[b], S)) < last) continue;     // its best
+        const T* row = logits + (entry * beams + b) * ldx;
+        for (int64_t t0 = 0; t0 < V && found < width; t0 += BM_THREADS * BM_AGAIN) {
+            const int64_t t1 = t0 + threadIdx.x * BM_AGAIN;
+            uint32_t hits = 0;
+#pragma unroll
+            for (int j = 0; j < BM_AGAIN; ++j) {
+                const int64_t t = t1 + j;
+                if (t >= V) continue;
+                const float v = done[b] ? finished_score(t == eos, S) : beam_score(clean(to_f32(row[t])), m[b], l[b], S);
+                hits |= v == last ? 1u << j : 0u;
+            }
+            if (!__syncthreads_or(hits != 0)) continue;
+            int place = __popc(hits);                       // inclusive sum over the lanes, then the warps
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, place, o);
+                if (lane >= o) place += v;
+            }
+            if (lane == 31) sums[warp] = place;
+            __syncthreads();
+            int all = 0, before = 0;
+            for (int q = 0; q < BM_WARPS; ++q) {
+                if (q == warp) before = all;
+                all += sums[q];
+            }
+            place += found + before - __popc(hits);
+            for (; hits && place < width; hits &= hits - 1, ++place) {
+                const int64_t t = t1 + __ffs(hits) - 1, o = entry * width + place;
+                out_scores[o] = last;
+                parents[o] = b;
+                tokens[o] = t;
+                if (out_finished) out_finished[o] = done[b] || t == eos;
+            }
+            found += all;
+            __syncthreads();                                // sums are written again
         }
     }
 }
@@ -147,8 +215,10 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
     uint64_t* best = own.key + items * width + (items * width & 1); // [warps][width]
     own.m = reinterpret_cast<float*>(best + BM_WARPS * width);
     own.s = own.m + items;
-    float* beam_m = own.s + items;                                  // [beams] maximum, log of the sum
+    own.out = reinterpret_cast<uint32_t*>(own.s + items);
+    float* beam_m = own.s + 2 * items;                              // [beams] maximum, log of the sum
     float* beam_l = beam_m + beams;
+    uint32_t* beam_out = reinterpret_cast<uint32_t*>(beam_l + beams);   // [beams] largest logit in no list
 
     __shared__ float own_score[BM_MAX];         // the entry's beams, read here for the join
     __shared__ uint8_t own_done[BM_MAX];
@@ -170,6 +240,7 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
         volatile uint32_t* floor = &floors[parts > 1 ? b - rank * BM_WARPS / parts : warp];
         if (parts == 1) *floor = 0;
         uint64_t list = 0;                                          // lane i: the i-th best so far
+        uint32_t out = 0;                                           // the lane's largest logit that was left out
         float m = -CUDART_INF_F, s = 0.0f;
         if (done) {
             // eos at the beam's own score, the other tokens masked: the first part lists them
@@ -216,7 +287,10 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
                 // the lanes' maxima (so many logits reach that).
                 uint64_t bar = __shfl_sync(0xffffffffu, list, width - 1);
                 uint32_t reach = max((uint32_t)(bar >> 32), *floor);
-                if (!__any_sync(0xffffffffu, valid && ordered(top) >= reach)) continue;
+                if (!__any_sync(0xffffffffu, valid && ordered(top) >= reach)) {
+                    out = max(out, ordered(top));
+                    continue;
+                }
                 if (bar == 0) {
                     uint32_t t = valid ? ordered(top) : 0u, low = 0;
                     for (int n = 0; n < width; ++n) {
@@ -230,9 +304,14 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
                 }
                 const float least = reach ? unordered(reach) : -CUDART_INF_F;
                 uint32_t left = 0;
+                float below = -CUDART_INF_F;
 #pragma unroll
-                for (int i = 0; i < BM_PER; ++i) left |= x[i] >= least ? 1u << i : 0u;
+                for (int i = 0; i < BM_PER; ++i) {
+                    if (x[i] >= least) left |= 1u << i;
+                    else below = fmaxf(below, x[i]);
+                }
                 left &= valid;
+                out = max(out, ordered(below));
                 // the few that qualify are read again (from L1): short code, because a step of
                 // few beams mostly waits for instructions
                 while (__any_sync(0xffffffffu, left != 0)) {
@@ -244,6 +323,7 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
                         k = cand_key(clean(to_f32(row[at])), (uint32_t)at);
                     }
                     const uint32_t in = __ballot_sync(0xffffffffu, k > bar);
+                    if (k <= bar) out = max(out, (uint32_t)(k >> 32));
                     if (in == 0) continue;
                     // the place of every candidate and every list entry is the number of keys
                     // that beat it: all are counted side by side (inserted one by one, each
@@ -265,7 +345,11 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
                     }
                     __syncwarp();
                     if (moved < width) scratch[BM_LIST + moved] = list;
-                    if (k > bar && place < width) scratch[BM_LIST + place] = k;
+                    else out = max(out, (uint32_t)(list >> 32));
+                    if (k > bar) {
+                        if (place < width) scratch[BM_LIST + place] = k;
+                        else out = max(out, (uint32_t)(k >> 32));
+                    }
                     __syncwarp();
                     list = lane < width ? scratch[BM_LIST + lane] : 0;
                     bar = scratch[BM_LIST + width - 1];
@@ -281,6 +365,7 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
         float sw = m > -CUDART_INF_F ? s * exp2_fast(-rounding_of(m)) * exp_fast(m - mw) : 0.0f;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sw += __shfl_xor_sync(0xffffffffu, sw, o);
+        out = __reduce_max_sync(0xffffffffu, out);
         if (!waited) {
             cluster.barrier_wait(std::move(started));
             waited = true;
@@ -290,6 +375,7 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
         if (lane == 0) {
             *cluster.map_shared_rank(own.m + item, 0) = mw;
             *cluster.map_shared_rank(own.s + item, 0) = sw;
+            *cluster.map_shared_rank(own.out + item, 0) = out;
         }
     }
     if (!waited) cluster.barrier_wait(std::move(started));
@@ -298,7 +384,12 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
 
     for (int b = warp; b < beams; b += BM_WARPS) {
         float m = -CUDART_INF_F;
-        for (int i = b * parts + lane; i < (b + 1) * parts; i += 32) m = fmaxf(m, own.m[i]);
+        uint32_t out = 0;
+        for (int i = b * parts + lane; i < (b + 1) * parts; i += 32) {
+            m = fmaxf(m, own.m[i]);
+            out = max(out, own.out[i]);
+        }
+        out = __reduce_max_sync(0xffffffffu, out);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         float s = 0.0f;
@@ -306,7 +397,7 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
             if (own.m[i] > -CUDART_INF_F) s += own.s[i] * exp_fast(own.m[i] - m);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) { beam_m[b] = m; beam_l[b] = logf(s); }
+        if (lane == 0) { beam_m[b] = m; beam_l[b] = logf(s); beam_out[b] = out; }
     }
     __syncthreads();
     // logits -> scores, in place; the index of (beam, token) is beam V + token
@@ -316,8 +407,7 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
         uint64_t r = 0;
         if (k != 0) {
             const float S = own_score[b], x = unordered((uint32_t)(k >> 32));
-            float v = own_done[b] ? x + S : beam_m[b] > -CUDART_INF_F ? (x - beam_m[b]) - beam_l[b] + S : -CUDART_INF_F;
-            if (v != v) v = -CUDART_INF_F;
+            const float v = own_done[b] ? finished_score(x == 0.0f, S) : beam_score(x, beam_m[b], beam_l[b], S);
             r = cand_key(v, (uint32_t)b * (uint32_t)V + ~(uint32_t)k);
         }
         own.key[i] = r;
@@ -340,7 +430,10 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
         }
     }
     __syncthreads();
+    __shared__ float last_score;
+    __shared__ int sums[BM_WARPS];
     const int total = BM_WARPS * width;                             // at most one per thread
+    float mine = -CUDART_INF_F;
     if (threadIdx.x < total) {
         const uint64_t k = best[threadIdx.x];
         int place = 0;
@@ -353,12 +446,25 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
             const uint32_t at = ~(uint32_t)k;
             const int b = (int)(at / (uint32_t)V);
             const int64_t t = at - (uint32_t)b * (uint32_t)V, o = entry * width + place;
-            out_scores[o] = unordered((uint32_t)(k >> 32));
+            mine = unordered((uint32_t)(k >> 32));
+            if (place == width - 1) last_score = mine;
+            out_scores[o] = mine;
             parents[o] = b;
             tokens[o] = t;
             if (out_finished) out_finished[o] = own_done[b] || t == eos;
         }
     }
+    __syncthreads();
+    // A candidate in no list is no better than `width` of its beam's that are in one, so it can
+    // only matter with the very score of the last chosen one.
+    const float last = last_score;
+    bool missed = last == -CUDART_INF_F;
+    if (threadIdx.x < beams && !own_done[threadIdx.x] && beam_out[threadIdx.x])
+        missed |= beam_score(unordered(beam_out[threadIdx.x]), beam_m[threadIdx.x], beam_l[threadIdx.x], own_score[threadIdx.x]) >= last;
+    if (!__syncthreads_or(missed)) return;
+    const int better = __syncthreads_count(mine > last);
+    choose_equal<T>(logits, V, ldx, beams, entry, own_score, own_done, beam_m, beam_l, eos, width, last, better, sums,
+                    out_scores, parents, tokens, out_finished);
 }
 
 template <typename T>

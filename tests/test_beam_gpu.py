@@ -320,3 +320,89 @@ def test_reorder_packed_with_more_beams_than_a_step_has(B, k, w):
     want = bits[_src(parents, k)].contiguous()
     assert torch.equal(_hard.unpack(got, B * w), want)
     assert torch.equal(got, _hard.pack(want, ldw=got.shape[1]))
+
+
+def _exact_order(x, scores, finished, eos, width):
+    """The step in 32 bits for rows whose normaliser is exactly 1 (one logit far above the
+    others): scores are then single roundings, which torch reproduces bit for bit."""
+    B, k = scores.shape
+    V = x.shape[-1]
+    x = x.float().view(B, k, V)
+    c = (x - x.amax(2, keepdim=True)) + scores[:, :, None]
+    c = torch.where(torch.isnan(c), NEG, c)
+    if finished is not None:
+        only = torch.full_like(c, NEG)
+        only[:, :, eos] = scores
+        c = torch.where(finished[:, :, None], only, c)
+    v, i = torch.sort(c.view(B, k * V), dim=1, descending=True, stable=True)
+    return v[:, :width], i[:, :width]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("B,k,width,V", [(1, 1, 1, 50), (1, 1, 1, 40000), (3, 1, 4, 1023), (1, 4, 4, 20001), (70, 4, 4, 3000),
+                                         (2, 8, 8, 9000), (1, 32, 32, 2000), (5, 3, 32, 700), (200, 2, 2, 2500)])
+@pytest.mark.parametrize("size", [30.0, 3e4, 2e6, 1e9])
+def test_equal_scores_of_different_logits_go_to_the_lowest_index(B, k, width, V, dtype, size):
+    """Far from zero, scores of different logits round to the same value: the order is that of
+    the rounded scores, then of the indices."""
+    g = torch.Generator().manual_seed(V + B)
+    x = -150.0 - 150.0 * torch.rand(B * k, V, generator=g)
+    x[torch.arange(B * k), torch.randint(0, V, (B * k,), generator=g)] = 0.0     # the normaliser is 1
+    x[torch.rand(B * k, V, generator=g) < 0.1] = NEG
+    x[torch.arange(B * k), torch.randint(0, V, (B * k,), generator=g)] = 0.0
+    top = (x == 0).sum(1) > 1
+    x[top] = torch.where(x[top] == 0, torch.where((x[top] == 0).cumsum(1) > 1, -200.0, 0.0), x[top])
+    x = x.to(dtype).to(dev)
+    scores = (-size * (1 + torch.randint(0, 3, (B, k), generator=g))).to(dev)
+    scores[torch.rand(B, k, generator=g).to(dev) < 0.1] = NEG
+    finished = (torch.rand(B, k, generator=g) < 0.2).to(dev)
+    for done, eos in ((None, None), (finished, V - 1)):
+        r = S.beam_step(x, scores, finished=done, eos=eos, width=width)
+        v, i = _exact_order(x, scores, done, eos, width)
+        assert torch.equal(r.scores, v)
+        assert torch.equal(r.parents * V + r.tokens, i)
+        if eos is not None:
+            assert torch.equal(r.finished, torch.gather(done, 1, r.parents) | (r.tokens == eos))
+
+
+@pytest.mark.parametrize("V", [2, 300, 5000, 40001])
+@pytest.mark.parametrize("B", [1, 64, 300])
+def test_neighbouring_logits_whose_scores_are_equal(B, V):
+    """1 - 2^-24 and 1 are half a unit of the score apart at -20.69: token 0 wins."""
+    x = torch.full((B, V), -300.0, device=dev)
+    x[:, 0], x[:, V // 2] = 1 - 2.0 ** -24, 1.0
+    r = S.beam_step(x, torch.full((B, 1), -20.0, device=dev), width=2)
+    assert bool((r.scores == r.scores[0, 0]).all()) and abs(r.scores[0, 0].item() + 20.693148) < 1e-5
+    assert bool((r.tokens[:, 0] == 0).all()) and bool((r.tokens[:, 1] == V // 2).all())
+    r = S.beam_step(x, torch.full((B, 1), -20.0, device=dev))
+    assert bool((r.tokens == 0).all())
+
+
+@pytest.mark.parametrize("V", [3, 40, 3000, 20001])
+def test_entries_with_no_beam_in_use(V):
+    """Every candidate scores -inf: the lowest indices, whatever the logits."""
+    k = 3
+    x = torch.randn(4 * k, V, device=dev)
+    scores = torch.full((4, k), NEG, device=dev)
+    scores[3] = float("nan")                                    # a NaN score is no better
+    r = S.beam_step(x, scores)
+    assert bool((r.scores == NEG).all()) and bool((r.parents == 0).all())
+    assert torch.equal(r.tokens, torch.arange(k, device=dev).expand(4, k))
+    r = S.beam_step(x, scores, width=2 * V if V <= 16 else 32, eos=1)
+    at = r.parents * V + r.tokens
+    assert torch.equal(at, torch.arange(at.shape[1], device=dev).expand_as(at)) and torch.equal(r.finished, r.tokens == 1)
+    scores[1, 2] = -4.0                                         # one beam in use, with one token allowed
+    x[5] = NEG
+    x[5, V - 1] = 2.0
+    r = S.beam_step(x, scores)
+    assert r.scores[1].tolist() == [-4.0, NEG, NEG] and r.parents[1].tolist() == [2, 0, 0]
+    assert r.tokens[1].tolist() == [V - 1, 0, 1]
+
+
+def test_unused_beams_at_a_large_negative_score():
+    """Beams parked at -1e9, as decoders do: candidates that fill a place tie and go by index."""
+    x = torch.randn(4, 2, device=dev)
+    scores = torch.tensor([[0.0, -1e9, -1e9, -1e9]], device=dev)
+    r = S.beam_step(x, scores, width=6)
+    assert sorted(r.tokens[0, :2].tolist()) == [0, 1] and r.parents[0, :2].tolist() == [0, 0]
+    assert (r.parents[0, 2:] * 2 + r.tokens[0, 2:]).tolist() == [2, 3, 4, 5]
