@@ -282,11 +282,15 @@ beam_step_kernel(const T* __restrict__ logits, int64_t V, int64_t ldx, int beams
                     for (int i = 0; i < BM_PER; ++i) t += exp_fast(x[i] - ref);
                     s = fmaf(t, factor, s);
                 }
-                // Logits that can be among the beam's best reach the last entry of any of its
-                // warps' lists; while a list is being filled, also the `width`-th largest of
-                // the lanes' maxima (so many logits reach that).
+                // Logits that can be among the beam's best pass the last entry of the warp's own
+                // list (an equal one is a later token), and reach that of the beam's other warps;
+                // while a list is being filled, also the `width`-th largest of the lanes' maxima
+                // (so many logits reach that).  With "reach" for the own list too, every unit of
+                // a row that is masked but for fewer tokens than `width` was searched: 64 against
+                // 37 us on 64 x 8 x 32,000 with 4 tokens allowed.
                 uint64_t bar = __shfl_sync(0xffffffffu, list, width - 1);
-                uint32_t reach = max((uint32_t)(bar >> 32), *floor);
+                uint32_t reach = *floor;
+                if (bar != 0) reach = max(reach, (uint32_t)(bar >> 32) + 1);
                 if (!__any_sync(0xffffffffu, valid && ordered(top) >= reach)) {
                     out = max(out, ordered(top));
                     continue;

@@ -406,3 +406,25 @@ def test_unused_beams_at_a_large_negative_score():
     r = S.beam_step(x, scores, width=6)
     assert sorted(r.tokens[0, :2].tolist()) == [0, 1] and r.parents[0, :2].tolist() == [0, 0]
     assert (r.parents[0, 2:] * 2 + r.tokens[0, 2:]).tolist() == [2, 3, 4, 5]
+
+
+@pytest.mark.parametrize("allowed", [0, 1, 3, 9])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16", "fp16"])
+def test_constrained_rows(allowed, dtype):
+    """All but a few tokens masked (fewer than there are beams): the allowed ones in order, then
+    what scores -inf by index; a constant row, whose logits all equal the last of its list."""
+    k, V, B = 4, 9001, 3
+    g = torch.Generator().manual_seed(allowed)
+    x = torch.full((B * k, V), NEG)
+    for r in range(B * k):
+        x[r, torch.randperm(V, generator=g)[:allowed]] = torch.randn(allowed, generator=g)
+    x[5] = 1.5
+    x = x.to(dtype).to(dev)
+    scores = -torch.rand(B, k, generator=g).to(dev)
+    r = _check(x, scores)
+    if allowed == 0:
+        assert (r.parents[0] * V + r.tokens[0]).tolist() == [0, 1, 2, 3]
+        assert r.parents[1].tolist() == [1] * 4 and r.tokens[1].tolist() == [0, 1, 2, 3]
+    if allowed == 1:
+        left = torch.isinf(r.scores[2])
+        assert int(left.sum()) == 0 and sorted(r.parents[2].tolist()) == [0, 1, 2, 3]
