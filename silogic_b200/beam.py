@@ -38,6 +38,10 @@ def beam_step(logits, scores, finished=None, eos=None, width=None):
         raise ValueError(f"beam_step: logits {tuple(logits.shape)} do not fit scores {tuple(scores.shape)}")
     if not (logits.is_cuda and scores.is_cuda and (finished is None or finished.is_cuda)):
         require_cuda(logits, scores, finished)
+    dev = logits.device
+    if scores.device != dev or finished is not None and finished.device != dev:
+        raise ValueError(f"beam_step: logits on {dev}, scores on {scores.device}, finished on "
+                         f"{finished.device if finished is not None else None}")
     width = beams if width is None else int(width)
     if not 1 <= beams <= BEAM_MAX or not 1 <= width <= BEAM_MAX:
         raise ValueError(f"beam_step: beams and width must be in 1..{BEAM_MAX}, got {beams} and {width}")
@@ -51,7 +55,6 @@ def beam_step(logits, scores, finished=None, eos=None, width=None):
         if finished.shape != scores.shape or finished.dtype not in (torch.bool, torch.uint8):
             raise ValueError("beam_step: finished must be bool, of the shape of scores")
         finished = finished.contiguous()
-    dev = logits.device
     x = logits if logits.dim() == 2 else logits.reshape(B * beams, V)
     if B and (x.stride(1) != 1 and V > 1 or x.stride(0) < V):
         x = x.contiguous()
@@ -79,6 +82,8 @@ def beam_reorder(state, parents, layout="rows", beams=None):
         raise ValueError("beam_reorder: parents must be [B, width] int64")
     if not (state.is_cuda and parents.is_cuda):
         require_cuda(state, parents)
+    if state.device != parents.device:
+        raise ValueError(f"beam_reorder: state on {state.device}, parents on {parents.device}")
     B, width = parents.shape
     parents = parents.contiguous()
     st = stream_ptr(state.device)

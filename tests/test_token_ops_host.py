@@ -197,3 +197,18 @@ def test_checkpoint8_is_read_again_by_a_traced_function():
         with S.checkpoint8(False):
             assert f(x)[0] == 6
     assert f(x)[0] == 6
+
+
+def test_beams_refuse_tensors_of_two_devices():
+    """Shapes alone (fake tensors): the devices are compared before anything is launched."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        make = lambda *s, d, t=torch.float32: torch.empty(s, device=f"cuda:{d}", dtype=t)      # noqa: E731
+        with pytest.raises(ValueError, match="scores on cuda:1"):
+            S.beam_step(make(4, 10, d=0), make(2, 2, d=1))
+        with pytest.raises(ValueError, match="finished on cuda:1"):
+            S.beam_step(make(4, 10, d=0), make(2, 2, d=0), finished=make(2, 2, d=1, t=torch.bool), eos=0)
+        for layout, state in (("rows", make(4, 7, d=0)), ("features", make(7, 4, d=0)),
+                              ("packed", make(7, 1, d=0, t=torch.int64))):
+            with pytest.raises(ValueError, match="parents on cuda:1"):
+                S.beam_reorder(state, make(2, 2, d=1, t=torch.int64), layout=layout)
