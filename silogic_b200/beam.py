@@ -78,8 +78,8 @@ def beam_reorder(state, parents, layout="rows", beams=None):
     fp32 ``[F, ldb]``; ``"packed"`` -- bit-packed ``[F, ldw]`` int64 words, sample s = bit
     ``s % 64`` of word ``s // 64``.  ``beams`` (default: ``width``; rows: from the shape) is
     the number of beams that the state holds per entry."""
-    if parents.dim() != 2 or parents.dtype != torch.int64:
-        raise ValueError("beam_reorder: parents must be [B, width] int64")
+    if parents.dim() != 2 or parents.dtype != torch.int64 or parents.shape[1] == 0:
+        raise ValueError(f"beam_reorder: parents must be [B, width] int64, got {tuple(parents.shape)} {parents.dtype}")
     if not (state.is_cuda and parents.is_cuda):
         require_cuda(state, parents)
     if state.device != parents.device:

@@ -212,3 +212,10 @@ def test_beams_refuse_tensors_of_two_devices():
                               ("packed", make(7, 1, d=0, t=torch.int64))):
             with pytest.raises(ValueError, match="parents on cuda:1"):
                 S.beam_reorder(state, make(2, 2, d=1, t=torch.int64), layout=layout)
+
+
+def test_reorder_refuses_entries_of_no_beams():
+    for layout, state in (("rows", torch.zeros(4, 7)), ("features", torch.zeros(7, 4)),
+                          ("packed", torch.zeros(7, 1, dtype=torch.int64))):
+        with pytest.raises(ValueError, match="parents"):
+            S.beam_reorder(state, torch.zeros(2, 0, dtype=torch.int64), layout=layout)
