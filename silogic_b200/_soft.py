@@ -41,8 +41,14 @@ def __getattr__(name):
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
-def _keep_checkpoint(ctx):
-    return checkpointing() and any(ctx.needs_input_grad[:3])
+def store_wanted():
+    """For a launch description, before ``apply``: a Function's forward runs with the grad mode
+    off, and ``needs_input_grad`` does not look at it."""
+    return checkpointing() and torch.is_grad_enabled()
+
+
+def _keep_checkpoint(ctx, meta):
+    return meta["keep8"] and any(ctx.needs_input_grad[:3])
 
 
 def _store(xt, meta):
@@ -121,7 +127,7 @@ def _fc_meta(layer, wire_r=0):
     _hard.check_index_range(cand, layer.in_dim, "LogicLayer candidates")
     return dict(cand=cand.contiguous(), K=K, ste=ste, node=NODE_ID[kind], arity=layer.arity,
                 gate_hard=gate_hard, inv_tau=inv_tau, out_dim=layer.out_dim,
-                wire_r=wire_r), params, conn
+                wire_r=wire_r, keep8=store_wanted()), params, conn
 
 
 class FCSoft(torch.autograd.Function):
@@ -140,7 +146,7 @@ class FCSoft(torch.autograd.Function):
         params = params.float().contiguous()
         connc = conn.float().contiguous() if conn is not None else None
         y = op("fc_soft_fwd")(xt, meta["cand"], connc, params, *FCSoft._args(meta))
-        ctx.ckpt = kept is not None or _keep_checkpoint(ctx)
+        ctx.ckpt = kept is not None or _keep_checkpoint(ctx, meta)
         if ctx.ckpt:        # the backward pass works from 8-bit codes; xt itself is let go
             ctx.save_for_backward(*(kept or _store(xt, meta)), params, connc)
             ctx.ldb = xt.shape[1]
@@ -181,7 +187,7 @@ class FCSoftRows(torch.autograd.Function):
         ctx.shape = x.shape
         B = x.shape[0]
         x, kept = x.reshape(B, -1), None
-        if 0 < B <= 65535 * 128 and _keep_checkpoint(ctx):      # the fused kernel's grid
+        if 0 < B <= 65535 * 128 and _keep_checkpoint(ctx, meta):      # the fused kernel's grid
             xt, *kept = op("to_feature_major_ckpt")(x, ldb_for(B))
         else:
             xt = op("to_feature_major")(x, ldb_for(B))
@@ -310,7 +316,7 @@ def _conv_meta(conv, wire_r=0, pool=1):
     inv_tau = 1.0 / conv.tau if kind == "walsh" else 1.0
     meta = dict(cand=cand, K=K, ste=ste, node=NODE_ID[kind], arity=conv.node_arity, depth=conv.d,
                 gate_hard=gate_hard, inv_tau=float(inv_tau), kernel=conv.kh, pad=conv.padding,
-                n_out=conv.n, wire_r=wire_r, pool=pool)
+                n_out=conv.n, wire_r=wire_r, pool=pool, keep8=store_wanted())
     return meta, params, conn
 
 
@@ -341,7 +347,7 @@ class ConvSoft(torch.autograd.Function):
         y, arg = op("conv_soft_fwd")(xt, C, H, W, meta["cand"], connc, params,
                                      *ConvSoft._args(meta),
                                    keep)
-        ctx.ckpt = _keep_checkpoint(ctx)
+        ctx.ckpt = _keep_checkpoint(ctx, meta)
         if ctx.ckpt:
             ctx.save_for_backward(*_store(xt, meta), params, connc, arg)
             ctx.ldb = xt.shape[1]

@@ -46,7 +46,7 @@ def _fc(x, cand, w, params, node, arity, inv_tau=1.0):
     from .. import _hard
     _hard.check_index_range(cand, IN, "candidate indices")
     meta = dict(cand=cand, K=K, ste=DIRECT_WEIGHTS, node=node, arity=arity, gate_hard=0,
-                inv_tau=float(inv_tau), out_dim=OUT, wire_r=0, batch=B)
+                inv_tau=float(inv_tau), out_dim=OUT, wire_r=0, batch=B, keep8=_soft.store_wanted())
     xt = ToFeatureMajor.apply(x.float())
     yt = FCSoft.apply(xt, params, w.float(), meta)
     return FromFeatureMajor.apply(yt, B).to(x.dtype)
@@ -103,7 +103,7 @@ def _conv(x, cm, ch, cw, w, params, node, arity, depth, stride, pad, Ho, Wo,
     _hard.check_index_range(cand, C * k * k, "conv leaf candidates")
     meta = dict(cand=cand, K=K, ste=DIRECT_WEIGHTS if w is not None else 0, node=node,
                 arity=arity, depth=depth, gate_hard=0, inv_tau=1.0, kernel=k, pad=pad, n_out=N,
-                wire_r=0, pool=1, batch=B)
+                wire_r=0, pool=1, batch=B, keep8=_soft.store_wanted())
     if deterministic:
         meta["deterministic"] = True
     xt = ToFeatureMajor.apply(x.reshape(B, -1).float())

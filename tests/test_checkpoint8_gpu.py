@@ -390,3 +390,24 @@ def test_a_single_layer_traces_under_torch_compile(on):
     assert torch.equal(y0, y1)
     for a, b in zip(torch.autograd.grad(y1, wanted, gy), torch.autograd.grad(y0, wanted, gy)):
         _close(a, b.double(), "compiled")
+
+
+def test_nothing_is_stored_without_a_backward_pass(monkeypatch):
+    """Under no_grad (evaluation inside a training context) no codes are written."""
+    from silogic_b200 import _ops
+    stored = []
+    for name in ("ckpt_store", "to_feature_major_ckpt"):
+        monkeypatch.setitem(_ops.IMPL, name, lambda *a, f=_ops.IMPL[name], n=name: (stored.append(n), f(*a))[1])
+    torch.manual_seed(0)
+    layer = S.LogicLayer(20, 30, node="walsh", k=4, seed=0).to(dev)
+    net = S.LogicNet(20, 30, 2, node="gate16", k=4, tau=3.0, seed=0).to(dev)
+    conv = S.ConvLogicTree(3, 8, tree_depth=2, k=4, seed=0).to(dev)
+    x, img = torch.rand(50, 20, device=dev), torch.rand(5, 3, 8, 8, device=dev)
+    with S.checkpoint8():
+        with torch.no_grad():
+            for f, v in ((layer, x), (net, x), (conv, img)):
+                f(v)
+        assert stored == []
+        for f, v in ((layer, x), (net, x), (conv, img)):
+            f(v)
+    assert stored == ["to_feature_major_ckpt", "ckpt_store", "ckpt_store", "ckpt_store"]
