@@ -7,6 +7,7 @@ Every Function's backward is a CUDA kernel too; parameter-side transforms
 (connection softmax, gate_probs @ basis, sigmoid of LUT logits) are fused into
 the layer kernels.
 """
+import functools
 import threading
 
 import torch
@@ -57,6 +58,31 @@ def _store(xt, meta):
     return op("ckpt_store")(xt if B is None or B == xt.shape[1] else xt[:, :B])
 
 
+# ------------------------------------------------------ gradients of gradients
+class _NoSecondOrder(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, g):
+        return g.view_as(g)
+
+    @staticmethod
+    def backward(ctx, gg):
+        raise RuntimeError("the soft layers of silogic_b200 have no second derivatives: a gradient taken with "
+                           "create_graph=True cannot be differentiated")
+
+
+def first_order(backward):
+    """The backward kernels' results carry no graph.  Under create_graph=True they are given one
+    that raises, so a loss that contains a gradient is refused instead of losing that term."""
+    @functools.wraps(backward)
+    def run(ctx, *g):
+        out = backward(ctx, *g)
+        if not torch.is_grad_enabled() or torch.compiler.is_compiling():
+            return out
+        mark = lambda t: None if t is None else _NoSecondOrder.apply(t.detach().requires_grad_())      # noqa: E731
+        return tuple(map(mark, out)) if isinstance(out, tuple) else mark(out)
+    return run
+
+
 # ------------------------------------------------------------- transposes
 class ToFeatureMajor(torch.autograd.Function):
     @staticmethod
@@ -67,6 +93,7 @@ class ToFeatureMajor(torch.autograd.Function):
         return op("to_feature_major")(x.reshape(B, -1), ldb_for(B))
 
     @staticmethod
+    @first_order
     def backward(ctx, g):
         return op("from_feature_major")(g, ctx.shape[0]).view(ctx.shape)
 
@@ -78,6 +105,7 @@ class FromFeatureMajor(torch.autograd.Function):
         return op("from_feature_major")(xt, B)
 
     @staticmethod
+    @first_order
     def backward(ctx, g):
         return op("to_feature_major")(g, ctx.ldb), None
 
@@ -156,6 +184,7 @@ class FCSoft(torch.autograd.Function):
         return y
 
     @staticmethod
+    @first_order
     def backward(ctx, gy):
         m = ctx.meta
         need_gx = bool(ctx.needs_input_grad[0])
@@ -194,6 +223,7 @@ class FCSoftRows(torch.autograd.Function):
         return op("from_feature_major")(FCSoft.forward(ctx, xt, params, conn, meta, kept), B)
 
     @staticmethod
+    @first_order
     def backward(ctx, gy):
         B = ctx.shape[0]
         gx, gparams, gconn, _ = FCSoft.backward(ctx, op("to_feature_major")(gy, ldb_for(B)))
@@ -235,6 +265,7 @@ class GroupSumSoft(torch.autograd.Function):
         return op("groupsum_soft_fwd")(xt, B, C, float(tau), int(ste))
 
     @staticmethod
+    @first_order
     def backward(ctx, g):
         W, ldb, tau = ctx.dims
         return op("groupsum_soft_bwd")(g, W, ldb, tau), None, None, None, None
@@ -357,6 +388,7 @@ class ConvSoft(torch.autograd.Function):
         return y
 
     @staticmethod
+    @first_order
     def backward(ctx, gy):
         if ctx.ckpt:        # the conv kernels read fp32 planes: one block's input at a time
             codes, bounds, params, connc, arg = ctx.saved_tensors
@@ -482,6 +514,7 @@ class OrPoolSoft(torch.autograd.Function):
         return op("or_pool_fwd")(x, size)
 
     @staticmethod
+    @first_order
     def backward(ctx, gy):
         (x,) = ctx.saved_tensors
         return op("or_pool_bwd")(x, gy, ctx.size), None
@@ -509,6 +542,7 @@ class ThermometerSoft(torch.autograd.Function):
         return op("thermo_soft_fwd")(x, thr)
 
     @staticmethod
+    @first_order
     def backward(ctx, g):
         x, thr = ctx.saved_tensors
         gx, gthr = op("thermo_soft_bwd")(x, thr, g, ctx.scale, bool(ctx.needs_input_grad[0]))

@@ -17,7 +17,27 @@ class _TokenEmbedding(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         (ids,) = ctx.saved_tensors
+        if torch.is_grad_enabled() and not torch.compiler.is_compiling():       # create_graph=True
+            return None, _EmbeddingGradient.apply(ids, g, *ctx.args), None, None
         return None, op("embed_bwd")(ids, g, *ctx.args), None, None
+
+
+class _EmbeddingGradient(torch.autograd.Function):
+    """The gradient as a (linear) function of the upstream one, for gradients of gradients."""
+
+    @staticmethod
+    def forward(ctx, ids, g, V, scale, padding_idx):
+        ctx.save_for_backward(ids)
+        ctx.args = (V, scale, padding_idx)
+        return op("embed_bwd")(ids, g, V, scale, padding_idx)
+
+    @staticmethod
+    def backward(ctx, ggw):
+        (ids,) = ctx.saved_tensors
+        V, scale, pad = ctx.args
+        rows = _TokenEmbedding.apply(ids, ggw, scale, pad)
+        counted = (ids >= 0) & (ids < V) & (ids != pad)         # the others add nothing to the gradient
+        return None, torch.where(counted.unsqueeze(-1), rows, 0.0), None, None, None
 
 
 def token_embedding(ids, weight, scale=1.0, padding_idx=None, check=False):

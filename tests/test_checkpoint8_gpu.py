@@ -411,3 +411,28 @@ def test_nothing_is_stored_without_a_backward_pass(monkeypatch):
         for f, v in ((layer, x), (net, x), (conv, img)):
             f(v)
     assert stored == ["to_feature_major_ckpt", "ckpt_store", "ckpt_store", "ckpt_store"]
+
+
+@pytest.mark.parametrize("on", [False, True])
+def test_second_derivatives_are_refused(on):
+    """A gradient taken with create_graph=True is right, and raises when it is differentiated (it
+    had no graph, and a penalty on it vanished from the loss without a word)."""
+    torch.manual_seed(0)
+    layer = S.LogicLayer(20, 30, node="walsh", k=4, seed=0).to(dev)
+    net = S.LogicNet(20, 30, 2, node="gate16", k=4, tau=3.0, seed=0).to(dev)
+    conv = S.ConvLogicTree(3, 8, tree_depth=2, k=4, seed=0).to(dev)
+    for f, shape in ((layer, (9, 20)), (net, (9, 20)), (conv, (5, 3, 8, 8))):
+        x = torch.rand(shape, device=dev, requires_grad=True)
+        wanted = [x] + list(f.parameters())
+
+        def loss():
+            with S.checkpoint8(on):
+                return (f(x) ** 2).sum()
+        plain = torch.autograd.grad(loss(), wanted)
+        graph = torch.autograd.grad(loss(), wanted, create_graph=True)
+        for a, b in zip(graph, plain):
+            assert a.requires_grad
+            _close(a.detach(), b.double(), "first derivative")
+        for g in graph:
+            with pytest.raises(RuntimeError, match="second derivatives"):
+                (loss() + (g ** 2).sum()).backward()

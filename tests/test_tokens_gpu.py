@@ -218,3 +218,35 @@ def test_traced_by_torch_compile():
     m.zero_grad()
     (m(ids) ** 2).sum().backward()
     assert torch.equal(got, m.weight.grad)
+
+
+@pytest.mark.parametrize("pad", [None, 3])
+def test_gradients_of_gradients(pad):
+    """A penalty on the embedding's gradient, and a third derivative, against torch's indexing in
+    64 bits.  The tolerance is 2^-18 of the sum of magnitudes: each value passes through at
+    most three 32-bit sums of at most 60 terms."""
+    V, D, N = 11, 6, 60
+    g = torch.Generator().manual_seed(4)
+    ids = torch.randint(-1, V + 1, (N,), generator=g).to(dev)
+    c = torch.randn(N, D, generator=g).to(dev)
+    inside = (ids >= 0) & (ids < V)
+    counted = inside & (ids != pad) if pad is not None else inside
+
+    def values(w, lookup):
+        y = torch.where(inside[:, None], lookup(w), 0.0)
+        loss = (c.to(w.dtype) * y ** 3).sum()
+        (gw,) = torch.autograd.grad(loss, w, create_graph=True)
+        total = loss + (gw ** 2).sum()
+        (g2,) = torch.autograd.grad(total, w, create_graph=True)
+        (g3,) = torch.autograd.grad((g2 * w.detach()).sum(), w)
+        return gw, g2, g3
+
+    def plain(w):
+        rows = torch.where(counted[:, None], w[ids.clamp(0, V - 1)], w.detach()[ids.clamp(0, V - 1)])
+        return 1.5 * rows
+    w = (torch.randn(V, D, generator=g).to(dev)).requires_grad_(True)
+    w64 = w.detach().double().requires_grad_(True)
+    got = values(w, lambda m: S.token_embedding(ids, m, scale=1.5, padding_idx=pad).nan_to_num(0.0))
+    want = values(w64, plain)
+    for a, b in zip(got, want):
+        assert bool(((a.double() - b).abs() <= 2.0 ** -18 * b.abs().max()).all())
