@@ -1,6 +1,7 @@
 """Token input: scaled embedding lookup with a gradient summed over sorted tokens."""
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import _hard
 from ._lib import require_cuda
@@ -70,6 +71,9 @@ def token_embedding(ids, weight, scale=1.0, padding_idx=None, check=False):
     ids = ids.contiguous()
     if weight.requires_grad and torch.is_grad_enabled():
         return _TokenEmbedding.apply(ids, weight, float(scale), pad)
+    if not torch.compiler.is_compiling() and forward_ad.unpack_dual(weight).tangent is not None:
+        # a Function refuses a tangent by itself; the kernel would drop it
+        raise RuntimeError("token_embedding: forward-mode differentiation is not implemented")
     return op("embed_fwd")(ids, weight.contiguous(), float(scale))
 
 

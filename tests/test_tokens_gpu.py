@@ -250,3 +250,18 @@ def test_gradients_of_gradients(pad):
     want = values(w64, plain)
     for a, b in zip(got, want):
         assert bool(((a.double() - b).abs() <= 2.0 ** -18 * b.abs().max()).all())
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(grad):
+    """A tangent must not be dropped silently, whether or not the weight takes a gradient."""
+    from torch.autograd import forward_ad
+    ids = torch.tensor([1, 0, 2], device=dev)
+    w = torch.randn(4, 8, device=dev)
+    with forward_ad.dual_level():
+        assert S.token_embedding(ids, w).shape == (3, 8)                # no tangent: an ordinary lookup
+        dual = forward_ad.make_dual(w.requires_grad_(grad), torch.ones(4, 8, device=dev))
+        with pytest.raises(RuntimeError):
+            S.token_embedding(ids, dual)
+        with torch.no_grad(), pytest.raises(RuntimeError):
+            S.token_embedding(ids, dual)
