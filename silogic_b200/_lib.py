@@ -109,6 +109,25 @@ def lib():
     return _lib
 
 
+_nodes = None
+
+
+def nodes():
+    """Load (once) and return the extension with the autograd nodes, bound to :func:`lib`."""
+    global _nodes
+    if _nodes is None:
+        L = lib()
+        try:
+            from . import _autograd
+        except ImportError as e:
+            raise SilogicError(f"silogic_b200/_autograd.so does not load ({e}): build it with "
+                               "`python -m silogic_b200.build`") from e
+        _autograd.bind(*(ctypes.cast(getattr(L, n), ctypes.c_void_p).value
+                         for n in ("slg_embed_fwd", "slg_embed_bwd", "slg_embed_bwd_workspace_bytes", "slg_last_error")))
+        _nodes = _autograd
+    return _nodes
+
+
 def _apply_env_tuning(L):
     """SLG_TUNING="key=value,..." sets ``slg_tuning_set`` knobs when the library loads
     (kernel variants; results are identical for every setting)."""

@@ -1,14 +1,15 @@
 """Token input: scaled embedding lookup with a gradient summed over sorted tokens."""
 import torch
 import torch.nn as nn
-from torch.autograd import forward_ad
 
 from . import _hard
-from ._lib import require_cuda
+from ._lib import nodes, require_cuda
 from ._ops import DTYPE_ID, op
 
 
 class _TokenEmbedding(torch.autograd.Function):
+    """The node that torch.compile traces (eager calls use the native one, ``csrc/autograd.cpp``)."""
+
     @staticmethod
     def forward(ctx, ids, weight, scale, padding_idx):
         ctx.save_for_backward(ids)
@@ -18,27 +19,7 @@ class _TokenEmbedding(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         (ids,) = ctx.saved_tensors
-        if torch.is_grad_enabled() and not torch.compiler.is_compiling():       # create_graph=True
-            return None, _EmbeddingGradient.apply(ids, g, *ctx.args), None, None
         return None, op("embed_bwd")(ids, g, *ctx.args), None, None
-
-
-class _EmbeddingGradient(torch.autograd.Function):
-    """The gradient as a (linear) function of the upstream one, for gradients of gradients."""
-
-    @staticmethod
-    def forward(ctx, ids, g, V, scale, padding_idx):
-        ctx.save_for_backward(ids)
-        ctx.args = (V, scale, padding_idx)
-        return op("embed_bwd")(ids, g, V, scale, padding_idx)
-
-    @staticmethod
-    def backward(ctx, ggw):
-        (ids,) = ctx.saved_tensors
-        V, scale, pad = ctx.args
-        rows = _TokenEmbedding.apply(ids, ggw, scale, pad)
-        counted = (ids >= 0) & (ids < V) & (ids != pad)         # the others add nothing to the gradient
-        return None, torch.where(counted.unsqueeze(-1), rows, 0.0), None, None, None
 
 
 def token_embedding(ids, weight, scale=1.0, padding_idx=None, check=False):
@@ -69,11 +50,10 @@ def token_embedding(ids, weight, scale=1.0, padding_idx=None, check=False):
     if check:
         _hard.check_index_range(ids, V, "token ids")
     ids = ids.contiguous()
+    if not torch.compiler.is_compiling():
+        return nodes().token_embedding(ids, weight, float(scale), pad)
     if weight.requires_grad and torch.is_grad_enabled():
         return _TokenEmbedding.apply(ids, weight, float(scale), pad)
-    if not torch.compiler.is_compiling() and forward_ad.unpack_dual(weight).tangent is not None:
-        # a Function refuses a tangent by itself; the kernel would drop it
-        raise RuntimeError("token_embedding: forward-mode differentiation is not implemented")
     return op("embed_fwd")(ids, weight.contiguous(), float(scale))
 
 

@@ -265,3 +265,47 @@ def test_forward_mode_is_refused(grad):
             S.token_embedding(ids, dual)
         with torch.no_grad(), pytest.raises(RuntimeError):
             S.token_embedding(ids, dual)
+
+
+def test_eager_calls_run_on_the_native_node():
+    """A Python autograd Function cost a small training step more than its kernels; what such a
+    Function gives must hold for the native node too."""
+    V, D = 40, 24
+    ids, w, gy = _case(V, D, 30, torch.float32)
+    w.requires_grad_(True)
+    y = S.token_embedding(ids, w, scale=2.0)
+    assert not isinstance(y.grad_fn, torch.autograd.function.BackwardCFunction)
+    ids += 1                                                    # the backward pass would see other ids
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, w, gy)
+    ids -= 1
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(t) or t, lambda t: t):
+        y = S.token_embedding(ids, w, scale=2.0)
+    assert len(seen) == 1 and torch.equal(seen[0], ids)
+    (gw,) = torch.autograd.grad(y, w, gy, retain_graph=True)
+    _check_grad(gw, ids, gy, V, 2.0)
+    assert torch.equal(torch.autograd.grad(y, w, gy)[0], gw)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, w, gy)
+    for off in (torch.no_grad, torch.inference_mode):
+        with off():
+            z = S.token_embedding(ids, w, scale=2.0)
+        assert not z.requires_grad and torch.equal(z, y)
+    assert not S.token_embedding(ids, w.detach()).requires_grad
+    h = S.token_embedding(ids, w.half(), scale=2.0)             # a cast inside the graph
+    h.sum().backward()
+    assert w.grad.dtype == torch.float32 and bool((w.grad[ids] != 0).all())
+
+
+def test_backward_of_an_unused_and_of_a_partly_used_lookup():
+    ids, w, _ = _case(20, 8, 12, torch.float32)
+    w.requires_grad_(True)
+    a, b = S.token_embedding(ids, w), S.token_embedding(ids, w)
+    (gw,) = torch.autograd.grad(a[:5].sum(), w)                 # a gradient with zero rows
+    want = torch.zeros_like(gw).index_add_(0, ids[:5], torch.ones(5, 8, device=dev))
+    assert torch.equal(gw, want)
+    b.sum().backward()
+    b2 = S.token_embedding(ids, w)
+    b2.sum().backward()                                         # accumulates
+    assert torch.equal(w.grad, 2 * torch.zeros_like(gw).index_add_(0, ids, torch.ones(12, 8, device=dev)))
