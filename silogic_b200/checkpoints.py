@@ -66,8 +66,9 @@ def checkpoint8_store(x):
 def checkpoint8(enabled=True):
     """Layers run inside keep their inputs for the backward pass as 8-bit codes
     (``enabled=False`` switches it off inside).  The setting is the calling thread's: other
-    threads are not affected, and a thread started inside begins with it off.  The innermost
-    context that is still open decides."""
+    threads are not affected, and a thread started inside begins with it off (so does a forward
+    pass that autograd repeats in its own thread: enter the context inside the repeated
+    function).  The innermost context that is still open decides."""
     mine = [bool(enabled)]          # an object of its own: contexts may end in any order
     opened = _soft._switch.__dict__.setdefault("opened", [])
     opened.append(mine)

@@ -13,8 +13,8 @@
 // are laid out in shared memory and added to the rows by bulk reductions: one instruction
 // per candidate, where vector atomics from registers take 16 passes of the load/store unit's
 // data pipe each and made it the bound (81% busy).  10,000 nodes x 10,000 inputs x 4,096
-// samples, Top-8 Walsh: 481 us (335 without gx, 606 with vector atomics); the fp32 kernel
-// takes 680 (423 without gx).  What is left is instruction issue (about 800 per warp and
+// samples, Top-8 Walsh: 486 us (352 without gx, 606 with vector atomics); the fp32 kernel
+// takes 622 (391 without gx).  What is left is instruction issue (about 800 per warp and
 // block) and, for gx, 2.6 GB of additions in L2, whose units alone would take 230 us.
 #include "fc_soft_impl.cuh"
 

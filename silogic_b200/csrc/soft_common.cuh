@@ -194,15 +194,16 @@ __device__ __forceinline__ void node_bwd(const float* __restrict__ np, const flo
 // exponential is taken by its own lane, and sums run over the lanes' values in index order
 // by shuffles -- the order, and so the bits, of a serial loop.
 
-// Transform one node's raw parameters into np[] (see header).  Executed by one warp
-// cooperatively; `raw` = node parameter row.  gate_hard: STE one-hot gate in the forward
-// value.  Returns after __syncwarp.
+// The lane's value of a node's parameter row (0 past its end)
 template <int NODE, int AR>
 __device__ __forceinline__ float node_param_first(const float* __restrict__ raw, int lane) {
     constexpr int N = NODE == N_GATE16 ? 16 : NodeSize<NODE, AR>::NPG;
     return lane < N ? raw[lane] : 0.0f;
 }
 
+// Transform one node's raw parameters into np[] (see header).  Executed by one warp
+// cooperatively; `raw` = node parameter row.  gate_hard: STE one-hot gate in the forward
+// value.  Returns after __syncwarp.
 template <int NODE, int AR>
 __device__ __forceinline__ void stage_node_params(const float* __restrict__ raw, float first, float* np, int gate_hard,
                                                   float inv_tau, int lane) {

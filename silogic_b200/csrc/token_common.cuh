@@ -65,7 +65,7 @@ __device__ __forceinline__ uint4 pack16(const float* x) {
 
 inline bool aligned_to(const void* p, int64_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
-// Calls F.template operator()<T>() for an SLG_DT_* code; false when the code is unknown.
+// Calls f with a value of the element type of an SLG_DT_* code; false when the code is unknown.
 template <typename F>
 inline bool for_dtype(int dtype, F&& f) {
     switch (dtype) {
