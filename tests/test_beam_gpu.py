@@ -428,3 +428,23 @@ def test_constrained_rows(allowed, dtype):
     if allowed == 1:
         left = torch.isinf(r.scores[2])
         assert int(left.sum()) == 0 and sorted(r.parents[2].tolist()) == [0, 1, 2, 3]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("spread", [1e-6, 1e-4, 1e-2, 1.0, 8.0])
+@pytest.mark.parametrize("B,V,width", [(1, 33, 32), (3, 1024, 4), (150, 1000, 32), (300, 1025, 8), (2, 20000, 1), (64, 4097, 2)])
+def test_order_is_that_of_the_rounded_scores(B, V, width, spread, dtype):
+    """Bit for bit: a step at score 0 tells the normaliser l (its best token scores 0 - l); every
+    candidate's score is then three single roundings, (x - max) - l + S."""
+    g = torch.Generator().manual_seed(B + V)
+    x = (torch.randn(B, V, generator=g) * spread + 1.0)
+    x[torch.rand(B, V, generator=g) < 0.1] = NEG
+    x[:, V // 3] = 1.0
+    x = x.to(dtype).to(dev)
+    l = -S.beam_step(x, torch.zeros(B, 1, device=dev), width=1).scores
+    d = x.float() - x.float().amax(1, keepdim=True)
+    for size in (0.0, 1.0, 20.0, 1000.0, 1e5):
+        s = (-size * (1 + torch.rand(B, 1, generator=g))).to(dev)
+        r = S.beam_step(x, s, width=width)
+        v, i = torch.sort((d - l) + s, dim=1, descending=True, stable=True)
+        assert torch.equal(r.scores, v[:, :width]) and torch.equal(r.tokens, i[:, :width])
