@@ -117,7 +117,7 @@ __host__ __device__ inline int beam_parts(int cs, int beams, int units) {
     const int p = cs * BM_WARPS / beams;
     return p < 1 ? 1 : p < units ? p : units;
 }
-// at most 38,784 bytes (8 CTAs, 32 beams, width 32) beside 8,756 of fixed size
+// at most 38,784 bytes (8 CTAs, 32 beams, width 32) beside 8,752 of fixed size
 constexpr int BM_LIST = 34;             // candidates and a 0 before a warp's list in its scratch
 constexpr int BM_SCRATCH = BM_LIST + 32;
 static inline size_t beam_smem(int items, int beams, int width) {
